@@ -13,6 +13,8 @@ its own over the same kernels:
     MultiGlobalGraph                all heads in one GEMM -> attention -> cat_conv + cat_bn -> ReLU (+ dropout)   :103-130
     SingleGlobalGraph               one full-width head -> bn -> ReLU (+ dropout)                     :148-173
     GraphAttentionBlock             cat(x, local, global) as three K segments -> cat_conv + cat_bn -> ReLU      gast_net.py:22-33
+    TemporalAttention               [q | k | v] GEMM -> rotary -> decaying linear attention along the frames -> GEMM -> dropout +
+                                    residual + layer norm (gast_hip/temporal.py; no counterpart in the reference)
 
 Two paths per module.  Under torch.no_grad() (inference, feature extraction): the fused forward plans below (BatchNorm + ReLU applied
 in the consumers' load prologues, statistics from the producers' epilogues).  When autograd has to record the call (a parameter or the
@@ -379,3 +381,42 @@ def graph_attention_block_forward(mod, x):
     out = torch.empty(P, Co2, dtype=torch.float32, device=dev)
     ops.bnrelu_apply(O, P, Co2, sc, sh, out)
     return out.view(B, T, J, Co2).permute(0, 3, 1, 2).contiguous()
+
+
+# ------------------------------------------------------------------------------------------ TemporalAttention
+def _temporal_block(mod, x, positions, drop, attend):
+    """(B, T, J, C) -> (B, T, J, C); attend(q, k, v) is the attention: the whole sequence, or one frame on a state"""
+    from gast_hip.autograd_ops import Gemm
+    from gast_hip.temporal import add_layer_norm, rotary
+    B, T, J, C = x.shape
+    dom, H = (B, T, J), mod.heads
+    qkv = Gemm.apply(x.reshape(B * T * J, C), mod.qkv.weight, mod.qkv.bias, dom).view(B, T, J, 3, H, C // H)
+    q, k, v = qkv.unbind(3)                               # (views: the operators read the GEMM's output where it is)
+    freqs = mod.freqs(x.device)
+    if freqs is not None:
+        q, k = rotary((q, k), positions, freqs)
+    o = attend(q, k, v)
+    y = Gemm.apply(o.reshape(B * T * J, C), mod.out.weight, mod.out.bias, dom).view(B, T, J, C)
+    return add_layer_norm(y, x, mod.norm.weight, mod.norm.bias, eps=mod.norm.eps, drop=drop, salt=4)[0]
+
+
+@_on_input_device
+def temporal_attention_forward(mod, x, lengths=None):
+    """TemporalAttention.forward: x (B, T, J, C) -> (B, T, J, C)"""
+    from gast_hip.temporal import decay_attention
+    x = _check(mod, x, 4)
+    positions = torch.arange(x.shape[1], device=x.device)
+    drop = _drop_state(mod.dropout, mod.training, x.device)
+    return _temporal_block(mod, x, positions, drop, lambda q, k, v: decay_attention(q, k, v, mod.log_decay, lengths=lengths))
+
+
+@_on_input_device
+def temporal_attention_step(mod, x, state, active=None):
+    """TemporalAttention.step: x (B, J, C) -> (B, J, C); the streams of `active` (None: all) move on by a frame"""
+    from gast_hip.temporal import decay_attention_step
+    x = _check(mod, x, 3)
+    with torch.no_grad():
+        y = _temporal_block(mod, x.unsqueeze(1), state.position, None,
+                            lambda q, k, v: decay_attention_step(q[:, 0], k[:, 0], v[:, 0], mod.log_decay, state.S, lengths=active).unsqueeze(1))
+        state.position += 1 if active is None else active.clamp(0, 1).view(-1, 1)
+    return y.squeeze(1)

@@ -494,6 +494,61 @@ int gast_chunk_gather(const float* poses2d, const float* poses3d, const float* c
                       long first_pair, int B, int chunk, int pad, int causal_shift, int J2, int F2, int J3, int F3, int ncam,
                       const int32_t* perm2d, const int32_t* perm3d, float* out2d, float* out3d, float* outcam, gast_stream_t stream);
 
+/* ---- sequence operators (gast_hip/temporal.py): rotary positions, linear attention with a decay, layer norm ------------------
+ * These have no counterpart in the reference: they let a model on this framework look further back than the receptive field of
+ * the dilated convolutions.  A tensor is (B, T, J, H, D): a sequence belongs to one joint of one clip, J = 1 for plain tokens.
+ * Strides are in elements and free (a stride of 0 shares a head), the D channels of a head are contiguous. */
+typedef struct { void* p; long b, t, j, h; } gast_seq;
+
+/* y = x with channel pairs (f, f + R/2), or interleaved (2f, 2f + 1), turned by positions[b][t] * freqs[f], f < R/2, and multiplied by
+ * `scale`; channels R .. D-1 are copied.  positions: int32 (pos64 = 0) or int64 with strides pos_b (0: one row for all clips), pos_t.
+ * backward != 0: turned back (the gradient).  y may be x.  D <= GAST_ROTARY_MAX_D; n jobs (q and k) in one launch. */
+#define GAST_ROTARY_MAX_BATCH 4
+#define GAST_ROTARY_MAX_D 1024
+typedef struct { gast_seq x, y; int H; } gast_rotary_job;
+int gast_rotary_multi(int dtype, const gast_rotary_job* jobs, int n, int B, int T, int J, int D, int R, int interleaved, const void* positions,
+                      int pos64, long pos_b, long pos_t, const double* freqs, float scale, int backward, gast_stream_t stream);
+
+/* Layer norm of the rows of S, or of S = residual + drop(X) (residual != null; S is then written, rounded to the activation type, and
+ * the norm is of the rounded values): y = (s - mean) * rstd * gamma + beta, rstd = 1 / sqrt(var + eps).  gamma, beta: fp32 or null.
+ * mean, rstd: fp32 [rows], or null where no backward pass follows.  Dropout: the library's stream of tensor `salt` at element r * C + c
+ * (beyond 2^33 elements the high word enters the key); use_drop needs a residual.  ld*: row strides in elements. */
+int gast_layer_norm_fwd(int dtype, const void* X, long ldx, const void* residual, long ldr, long rows, int C, const float* gamma,
+                        const float* beta, float eps, int use_drop, uint32_t salt, gast_dropout drop, void* S, long lds, void* Y, long ldy,
+                        float* mean, float* rstd, gast_stream_t stream);
+/* dS = dStream + rstd * (dxhat - mean(dxhat) - xhat mean(dxhat xhat)), dxhat = dY gamma; dX = dS * dropout multiplier; dgamma, dbeta
+ * (null: not wanted) are written, summed in a fixed order.  dY or dStream may be null (zero).  dS null: not wanted; dX null: not wanted
+ * (without a residual pass dS only).  ws: gast_layer_norm_bwd_ws_floats(rows, C) floats, needed where dgamma or dbeta is. */
+int gast_layer_norm_bwd(int dtype, const void* dY, long lddy, const void* dStream, long ldds, const void* S, long lds, long rows, int C,
+                        const float* gamma, const float* mean, const float* rstd, int use_drop, uint32_t salt, gast_dropout drop, void* dX,
+                        long lddx, void* dS, long lddsum, float* dgamma, float* dbeta, float* ws, gast_stream_t stream);
+long gast_layer_norm_bwd_ws_floats(long rows, int C);
+
+/* Causal linear attention with a decay for each head, lambda_h = exp(log_decay[h]):
+ *   S_t = lambda S_(t-1) + k_t v_t',   o_t = scale q_t' S_t,   t < lengths[b] (null: T; clamped to 0 .. T)
+ * S_(-1) = state ([B][J][H][Dk][Dv] fp32; null: zero), state_out (null: not wanted) = S behind the last token.  Outputs behind a
+ * sequence's end are zero.  Dk, Dv <= GAST_DECAY_MAX_D. */
+#define GAST_DECAY_MAX_D 128
+typedef struct {
+    int dtype, B, T, J, H, Dk, Dv;
+    float scale;
+    const float* log_decay;      /* [H] */
+    const int32_t* lengths;      /* [B] or null */
+    gast_seq q, k, v, o;
+    const float* state;
+    float* state_out;
+    /* backward: o is not read; d_o in, dq, dk, dv out (zero behind a sequence's end); dstate_out (null: zero) in, dstate out (null: not wanted) */
+    gast_seq d_o, dq, dk, dv;
+    const float* dstate_out;
+    float* dstate;
+    float* ws;                   /* gast_decay_ws_floats() floats (null where that is 0) */
+} gast_decay_args;
+int gast_decay_fwd(const gast_decay_args* args, gast_stream_t stream);
+int gast_decay_bwd(const gast_decay_args* args, gast_stream_t stream);
+long gast_decay_ws_floats(int B, int T, int J, int H, int Dk, int Dv, int backward);
+/* One token of every stream: T = 1, state updated in place (state_out is ignored); streams with lengths[b] < 1 keep their state, o = 0. */
+int gast_decay_step(const gast_decay_args* args, gast_stream_t stream);
+
 /* launches an empty kernel: the fixed dispatch cost an event pair sees around any launch (bench.py calibration) */
 int gast_null_launch(gast_stream_t stream);
 const char* gast_version(void);
