@@ -7,97 +7,526 @@
 //   dv  a = k,  b = q,  c = do   backward in time           dk  a = v,  b = do, c = q    backward in time (X = the transposed one of dv)
 // Forward in time the carry is decayed before it is used (o_t sees lambda S_(t-1)), backward in time the gradient of the last state is
 // used as it is and the decay follows: d state = lambda * (the recurrence's end).
+#include <atomic>
 #include "seq_common.h"
 
 namespace {
 
-struct ScanArgs {
-    gast_seq a, b, c, out;
-    const float* xin;        // [B][J][H][D1][D2] (xin_t: [D2][D1]), or null: zero
-    float* xout;             // [B][J][H][D1][D2] or null
-    const float* log_decay;
-    const int32_t* lengths;
-    int B, T, J, H, D1, D2, xin_t, reverse;
-    float bscale, oscale;
-};
+// ------------------------------------------------------------------------------------------------ whole sequences, by chunks of 32 tokens
+// Inside a chunk the recurrence is products of matrices (i, j tokens of the chunk, X the state before it, n its tokens):
+//   out_i = sum_j [j before or at i] lambda^|i-j| (a_i b_j) c_j + lambda^(steps to i) a_i X,     X' = lambda^n X + sum_j lambda^(steps from j) b_j c_j'
+// A wave owns 32 columns of X (and of c and out) and keeps them in accumulators; the waves of a block share a, b, c of the chunk in LDS.
+// The 32x32 matrix instructions leave result rows 8 (r / 4) + 4 (lane / 32) + r % 4 in register r and the column in lane % 32, and take
+// operands with the row (or column) in lane % 32 and any order of the summed index that both sides agree on.  Every operand here is held in
+// that same order -- 16 values a lane for 32 summed indexes -- so scores (summed over d, then over j) and states (made by a sum over j, then
+// summed over d) go from one product into the next without leaving their registers.  Only tokens pass through LDS, b and c turned on the way.
+// Scores are computed by every wave for itself: D / 16 of 11 D / 32 instructions at 128 channels, against a barrier and an LDS round trip.
+//
+// Arithmetic.  fp32: fp32 matrix instructions.  16 bits: products of stored values are exact in fp32; scores and states, which are fp32,
+// meet 16-bit operands as two bf16 parts (hi = bf16(x), lo = bf16(x - hi): 2^-17 relative), what enters a state as three (all 24 bits: states
+// are results in fp32); in the binary16 flavour the stored operand is split into two bf16 parts as well (exactly; binary16 parts of a state
+// would overflow at 65504).  States are fp32 throughout.
+constexpr int CT = 32;               // tokens of a chunk
+constexpr int TS = CT + 4;           // row pitch of the turned tiles (elements): rows start 18 / 36 banks apart, no two of a read collide
 
-constexpr int TS = 16;       // tokens staged at a time
-constexpr int EC = 64;       // columns of X that a block owns
+template <typename T> struct Frag;
+template <> struct Frag<float> { float x[16]; };
+template <> struct Frag<bf16_t> { uint4 x[2]; };
+struct Split { uint4 hi[2], lo[2]; };                  // x = hi + lo to 2^-17
+struct Parts { uint4 x[3][2]; };                       // x = x[0] + x[1] + x[2], all of its 24 bits
 
-// The recurrence as it stands: a block owns EC columns of one head's X; wave p holds rows 32 p .. 32 p + 31 of them in registers.
-template <typename T>
-__global__ void __launch_bounds__(256) scan_kernel(const ScanArgs p) {
-    __shared__ float sa[TS][GAST_DECAY_MAX_D], sb[TS][GAST_DECAY_MAX_D], sc[TS][EC], so[4][TS][EC];
-    const int tid = threadIdx.x, e = tid & 63, w = tid >> 6, D1 = p.D1, D2 = p.D2;
-    const int nct = (D2 + EC - 1) / EC, ct = blockIdx.x % nct, e0 = ct * EC;
-    const long hd = blockIdx.x / nct;                   // (b, j, h)
-    const int h = (int)(hd % p.H), j = (int)(hd / p.H % p.J);
-    const long b = hd / p.H / p.J;
-    const float lam = expf(p.log_decay[h]);
-    const int len = p.lengths ? min(max(p.lengths[b], 0), p.T) : p.T;
-    const bool col = e0 + e < D2;
-    float X[32];
+// 16 values of a row of an LDS tile: elements 8 q + 4 (lane / 32) + 0 .. 3, q = 0 .. 3
+__device__ __forceinline__ Frag<float> ld_frag(const float* row, int half) {
+    Frag<float> f;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-        const int d = w * 32 + i;
-        X[i] = 0.f;
-        if (p.xin && d < D1 && col) X[i] = p.xin[hd * D1 * D2 + (p.xin_t ? (long)(e0 + e) * D1 + d : (long)d * D2 + e0 + e)];
-        if (!p.reverse && len) X[i] *= lam;
+    for (int q = 0; q < 4; ++q) {
+        const float4 v = *(const float4*)(row + 8 * q + 4 * half);
+        f.x[4 * q] = v.x; f.x[4 * q + 1] = v.y; f.x[4 * q + 2] = v.z; f.x[4 * q + 3] = v.w;
     }
-    const T *A = (const T*)p.a.p + seq_at(p.a, b, 0, j, h), *Bp = (const T*)p.b.p + seq_at(p.b, b, 0, j, h), *Cp = (const T*)p.c.p + seq_at(p.c, b, 0, j, h);
-    T* O = (T*)p.out.p + seq_at(p.out, b, 0, j, h);
-    for (int t0 = 0; t0 < len; t0 += TS) {
-        const int n = min(TS, len - t0);
-        for (int i = tid; i < n * D1; i += 256) {
-            const int q = i / D1, d = i - q * D1, t = p.reverse ? len - 1 - t0 - q : t0 + q;
-            sa[q][d] = Elem<T>::ld(A + t * p.a.t + d);
-            sb[q][d] = Elem<T>::ld(Bp + t * p.b.t + d) * p.bscale;
-        }
-        for (int i = tid; i < n * EC; i += 256) {
-            const int q = i / EC, c = i - q * EC, t = p.reverse ? len - 1 - t0 - q : t0 + q;
-            sc[q][c] = e0 + c < D2 ? Elem<T>::ld(Cp + t * p.c.t + e0 + c) : 0.f;
-        }
-        __syncthreads();
-        for (int q = 0; q < n; ++q) {
-            const float c = sc[q][e];
-            float o = 0.f;
-            const bool decay = t0 + q > 0;
+    return f;
+}
+__device__ __forceinline__ Frag<bf16_t> ld_frag(const bf16_t* row, int half) {
+    Frag<bf16_t> f;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                const int d = w * 32 + i;
-                if (d < D1) {
-                    X[i] = fmaf(sb[q][d], c, decay ? lam * X[i] : X[i]);
-                    o = fmaf(sa[q][d], X[i], o);
-                }
-            }
-            so[w][q][e] = o;
-        }
-        __syncthreads();
-        for (int i = tid; i < n * EC; i += 256) {
-            const int q = i / EC, c = i - q * EC, t = p.reverse ? len - 1 - t0 - q : t0 + q;
-            if (e0 + c < D2) Elem<T>::st(O + t * p.out.t + e0 + c, p.oscale * (so[0][q][c] + so[1][q][c] + so[2][q][c] + so[3][q][c]));
-        }
+    for (int q = 0; q < 2; ++q) {
+        const uint2 a = *(const uint2*)(row + 16 * q + 4 * half), b = *(const uint2*)(row + 16 * q + 8 + 4 * half);
+        f.x[q] = make_uint4(a.x, a.y, b.x, b.y);
     }
-    for (long i = tid; i < (long)(p.T - len) * EC; i += 256) {
-        const long t = len + i / EC;
-        const int c = (int)(i % EC);
-        if (e0 + c < D2) Elem<T>::st(O + t * p.out.t + e0 + c, 0.f);
-    }
-    if (p.xout && col)
+    return f;
+}
+__device__ __forceinline__ void unpack(const Frag<float>& f, float (&v)[16]) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            const int d = w * 32 + i;
-            if (d < D1) p.xout[hd * D1 * D2 + (long)d * D2 + e0 + e] = p.reverse && len ? lam * X[i] : X[i];
-        }
+    for (int i = 0; i < 16; ++i) v[i] = f.x[i];
+}
+__device__ __forceinline__ void unpack(const Frag<bf16_t>& f, float (&v)[16]) {
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        h16x2_unpack(f.x[q].x, v[8 * q], v[8 * q + 1]); h16x2_unpack(f.x[q].y, v[8 * q + 2], v[8 * q + 3]);
+        h16x2_unpack(f.x[q].z, v[8 * q + 4], v[8 * q + 5]); h16x2_unpack(f.x[q].w, v[8 * q + 6], v[8 * q + 7]);
+    }
+}
+template <typename V> __device__ __forceinline__ Split split16(const V& v) {
+    Split s;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        uint2 h0, l0, h1, l1;
+        split_pair4<1>(v[8 * q], v[8 * q + 1], v[8 * q + 2], v[8 * q + 3], h0, l0);
+        split_pair4<1>(v[8 * q + 4], v[8 * q + 5], v[8 * q + 6], v[8 * q + 7], h1, l1);
+        s.hi[q] = make_uint4(h0.x, h0.y, h1.x, h1.y);
+        s.lo[q] = make_uint4(l0.x, l0.y, l1.x, l1.y);
+    }
+    return s;
 }
 
+// c += A B over 32 summed indexes, both as stored
+__device__ __forceinline__ void mma(f32x16& c, const Frag<bf16_t>& a, const Frag<bf16_t>& b) {
+    c = mfma_h16(a.x[0], b.x[0], c);
+    c = mfma_h16(a.x[1], b.x[1], c);
+}
+__device__ __forceinline__ void mma(f32x16& c, const Frag<float>& a, const Frag<float>& b) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.x[i], b.x[i], c, 0, 0, 0);
+}
+// c += A B with one side in fp32 (16 values in the same order): rows from the fp32 side (mma_fs) or from the stored one (mma_sf)
+template <typename V> __device__ __forceinline__ void mma_fs(f32x16& c, const V& a, const Frag<float>& b) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b.x[i], c, 0, 0, 0);
+}
+template <typename V> __device__ __forceinline__ void mma_sf(f32x16& c, const Frag<float>& a, const V& b) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.x[i], b[i], c, 0, 0, 0);
+}
+__device__ __forceinline__ Split stored_parts(const Frag<bf16_t>& f) {
+    float v[16];
+    unpack(f, v);
+    return split16(v);
+}
+template <typename V> __device__ __forceinline__ void mma_fs(f32x16& c, const V& av, const Frag<bf16_t>& b) {
+    const Split a = split16(av);
+#ifdef GAST_H16_F16
+    const Split p = stored_parts(b);
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        c = mfma_pair<1>(a.lo[q], p.hi[q], c);
+        c = mfma_pair<1>(a.hi[q], p.lo[q], c);
+        c = mfma_pair<1>(a.hi[q], p.hi[q], c);
+    }
+#else
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        c = mfma_pair<1>(a.lo[q], b.x[q], c);
+        c = mfma_pair<1>(a.hi[q], b.x[q], c);
+    }
+#endif
+}
+__device__ __forceinline__ void mma_sf(f32x16& c, const Frag<bf16_t>& a, const Split& b) {
+#ifdef GAST_H16_F16
+    const Split p = stored_parts(a);
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        c = mfma_pair<1>(p.hi[q], b.lo[q], c);
+        c = mfma_pair<1>(p.lo[q], b.hi[q], c);
+        c = mfma_pair<1>(p.hi[q], b.hi[q], c);
+    }
+#else
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        c = mfma_pair<1>(a.x[q], b.lo[q], c);
+        c = mfma_pair<1>(a.x[q], b.hi[q], c);
+    }
+#endif
+}
+template <typename V> __device__ __forceinline__ Parts parts16(const V& v) {
+    Parts s;
+    float w[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) w[i] = v[i];
+#pragma unroll
+    for (int k = 0; k < 3; ++k)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            uint32_t u[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                float &a = w[8 * q + 2 * e], &b = w[8 * q + 2 * e + 1];
+                u[e] = pack_bf16x2(a, b);
+                a -= __uint_as_float(u[e] << 16);           // (exact)
+                b -= __uint_as_float(u[e] & 0xffff0000u);
+            }
+            s.x[k][q] = make_uint4(u[0], u[1], u[2], u[3]);
+        }
+    return s;
+}
+__device__ __forceinline__ void mma_sf(f32x16& c, const Frag<bf16_t>& a, const Parts& b) {
+#ifdef GAST_H16_F16
+    const Split p = stored_parts(a);
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        c = mfma_pair<1>(p.hi[q], b.x[2][q], c);
+        c = mfma_pair<1>(p.lo[q], b.x[1][q], c);
+        c = mfma_pair<1>(p.hi[q], b.x[1][q], c);
+        c = mfma_pair<1>(p.lo[q], b.x[0][q], c);
+        c = mfma_pair<1>(p.hi[q], b.x[0][q], c);
+    }
+#else
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+#pragma unroll
+        for (int k = 2; k >= 0; --k) c = mfma_pair<1>(a.x[q], b.x[k][q], c);
+#endif
+}
+// the fp32 side of mma_sf, prepared once where several products share it: scores in two parts, what enters a state in three
+template <typename T> struct Prepared;
+template <> struct Prepared<float> {
+    float v[16];
+    __device__ __forceinline__ void set(const float (&x)[16]) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = x[i];
+    }
+};
+template <> struct Prepared<bf16_t> { Split v; __device__ __forceinline__ void set(const float (&x)[16]) { v = split16(x); } };
+template <typename T> struct Exact : Prepared<float> {};
+template <> struct Exact<bf16_t> { Parts v; __device__ __forceinline__ void set(const float (&x)[16]) { v = parts16(x); } };
+
+// The 32 x DP tokens of one tensor on their way from memory to LDS: 16 elements a thread of NW waves.  16 bits: 8 channels of two rows,
+// so that a turned word holds both; four lanes read 64 contiguous bytes and the turned words of a wave fall into 64 different banks.
+struct View { const void* p; long t; int D, al; };       // token 0 of the sequence, its stride, channels, 16-byte rows
+template <typename T> struct Stage;
+template <> struct Stage<bf16_t> {
+    uint4 x[2];
+    __device__ __forceinline__ void load(const View& s, int t0, int n, int wv, int lane) {
+        const int d = (wv * 4 + (lane & 3)) * 8, row = (lane >> 2) * 2;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            x[k] = make_uint4(0, 0, 0, 0);
+            if (row + k >= n || d >= s.D) continue;
+            const bf16_t* p = (const bf16_t*)s.p + (long)(t0 + row + k) * s.t + d;
+            if (s.al && d + 8 <= s.D) {
+                x[k] = *(const uint4*)p;
+            } else {
+                uint32_t w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    w[e] = d + 2 * e < s.D ? p[2 * e] : 0;
+                    if (d + 2 * e + 1 < s.D) w[e] |= (uint32_t)p[2 * e + 1] << 16;
+                }
+                x[k] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        }
+    }
+    template <int RS> __device__ __forceinline__ void rows(bf16_t* tile, int wv, int lane) const {
+        bf16_t* p = tile + (lane >> 2) * 2 * RS + (wv * 4 + (lane & 3)) * 8;
+#pragma unroll
+        for (int k = 0; k < 2; ++k, p += RS) {
+            *(uint2*)p = make_uint2(x[k].x, x[k].y);
+            *(uint2*)(p + 4) = make_uint2(x[k].z, x[k].w);
+        }
+    }
+    __device__ __forceinline__ void turned(bf16_t* tile, int wv, int lane) const {
+        uint32_t* p = (uint32_t*)(tile + (wv * 4 + (lane & 3)) * 8 * TS) + (lane >> 2);
+        const uint32_t a[4] = {x[0].x, x[0].y, x[0].z, x[0].w}, b[4] = {x[1].x, x[1].y, x[1].z, x[1].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            p[(2 * e) * (TS / 2)] = __builtin_amdgcn_perm(b[e], a[e], 0x05040100u);
+            p[(2 * e + 1) * (TS / 2)] = __builtin_amdgcn_perm(b[e], a[e], 0x07060302u);
+        }
+    }
+};
+template <> struct Stage<float> {
+    float4 x[4];
+    __device__ __forceinline__ void load(const View& s, int t0, int n, int wv, int lane) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int d = (wv * 8 + (lane & 3) + 4 * (k & 1)) * 4, row = (lane >> 2) + 16 * (k >> 1);
+            x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (row >= n || d >= s.D) continue;
+            const float* p = (const float*)s.p + (long)(t0 + row) * s.t + d;
+            if (s.al && d + 4 <= s.D) {
+                x[k] = *(const float4*)p;
+            } else {
+                x[k].x = p[0];
+                if (d + 1 < s.D) x[k].y = p[1];
+                if (d + 2 < s.D) x[k].z = p[2];
+                if (d + 3 < s.D) x[k].w = p[3];
+            }
+        }
+    }
+    template <int RS> __device__ __forceinline__ void rows(float* tile, int wv, int lane) const {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            *(float4*)(tile + ((lane >> 2) + 16 * (k >> 1)) * RS + (wv * 8 + (lane & 3) + 4 * (k & 1)) * 4) = x[k];
+    }
+    __device__ __forceinline__ void turned(float* tile, int wv, int lane) const {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            float* p = tile + (wv * 8 + (lane & 3) + 4 * (k & 1)) * 4 * TS + (lane >> 2) + 16 * (k >> 1);
+            p[0] = x[k].x; p[TS] = x[k].y; p[2 * TS] = x[k].z; p[3 * TS] = x[k].w;
+        }
+    }
+};
+
+// Y (32 columns of out by 32 tokens, the token in lane % 32) to memory by way of LDS, so that a row leaves in 16-byte pieces
 template <typename T>
-int scan(const ScanArgs& p, hipStream_t s) {
-    const long blocks = (long)p.B * p.J * p.H * ((p.D2 + EC - 1) / EC);
-    if (blocks > 0x7fffffffL) return GAST_ERANGE;
-    hipLaunchKernelGGL((scan_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, s, p);
-    GAST_CHECK_LAUNCH();
-    return 0;
+__device__ __forceinline__ void put_tile(const f32x16& Y, T* tile, T* O, long st, int t0, int n, int c0, int D, int al, int lane) {
+    constexpr int VE = 16 / sizeof(T), VR = 32 / VE;      // vectors of a row
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+        st4(tile + (lane & 31) * TS + 8 * q + 4 * (lane >> 5), make_float4(Y[4 * q], Y[4 * q + 1], Y[4 * q + 2], Y[4 * q + 3]));
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+    for (int k = 0; k < VR / 2; ++k) {
+        const int row = lane / VR + k * (64 / VR), e = (lane % VR) * VE;
+        if (row >= n || c0 + e >= D) continue;
+        const T* s = tile + row * TS + e;
+        T* p = O + (long)(t0 + row) * st + c0 + e;
+        if (al && c0 + e + VE <= D) {
+            const uint2 u = *(const uint2*)s, w = *(const uint2*)(s + VE / 2);
+            *(uint4*)p = make_uint4(u.x, u.y, w.x, w.y);
+        } else {
+            for (int x = 0; x < VE && c0 + e + x < D; ++x) p[x] = s[x];
+        }
+    }
+}
+// rows [t0, t1) of out are behind the sequence's end: zero (by nthr threads)
+template <typename T>
+__device__ __forceinline__ void put_zeros(T* O, long st, int t0, int t1, int D, int al, int tid, int nthr) {
+    constexpr int VE = 16 / sizeof(T);
+    const int nv = (D + VE - 1) / VE;
+    for (long i = tid; i < (long)(t1 - t0) * nv; i += nthr) {
+        const long t = i / nv;
+        const int e = (int)(i - t * nv) * VE;
+        T* p = O + (t0 + t) * st + e;
+        if (al && e + VE <= D) *(uint4*)p = make_uint4(0, 0, 0, 0);
+        else
+            for (int x = 0; x < VE && e + x < D; ++x) p[x] = (T)0;
+    }
+}
+
+// Which tensors a kernel stages and what its groups of DP / 32 waves do with them.
+//   ONE    in = a, b, c, one group                                                (o, and dq)
+//   TWO    in = q, do, k, v: group 0 makes dv, group 1 dk                         (both run backward in time)
+//   THREE  in = q, do, k, v: group 2 makes dq as well                             (sequences of one chunk: no state to hand on to dq)
+//   SUMS   in = -, b, c: only X, from zero, of each segment
+enum { ONE, TWO, THREE, SUMS };
+
+struct Role {
+    gast_seq out;
+    const float* xin;                // X before the first token in this direction, [head][segment][D1][D2], or null: zero
+    float* xout;                     // X behind the last, or null
+    int turn, reverse, D1, D2, al;   // turn: xin is held as [D2][D1]
+    float fp, fk, fo;                // factors of scores, of what enters X, of what the carried X gives
+};
+
+struct ChunkArgs {
+    gast_seq in[4];
+    int D[4], al[4];                 // channels; rows on 16 bytes
+    Role role[3];
+    const float* log_decay;
+    const int32_t* lengths;
+    int B, T, J, H, nseg, L, skip_last;     // segments of L tokens; skip_last: nobody reads the sums of the last one in this direction
+};
+
+// LDS of a kernel, in elements: tiles as rows, turned tiles, output tiles of the waves (ONE: over the wave's own columns of c)
+template <int DP, int MODE> struct Lay {
+    static constexpr int NW = DP / 32, RS = DP + 4, ROWS = CT * RS, TURN = DP * TS;
+    static constexpr int GROUPS = MODE == TWO ? 2 : MODE == THREE ? 3 : 1, NT = GROUPS * NW * 64;
+    static constexpr int NROWS = MODE == ONE ? 2 : MODE == SUMS ? 0 : 4, NTURN = MODE == THREE ? 3 : 2;
+    static constexpr int OUT = MODE == TWO || MODE == THREE ? GROUPS * NW * 32 * TS : 0;
+    static constexpr int ELEMS = NROWS * ROWS + NTURN * TURN + OUT;
+};
+
+struct Powers { float p[CT + 4], m[CT + 4]; };            // lambda^n, and lambda^n - 1
+
+template <typename T, int DP, int MODE>
+__global__ void __launch_bounds__((Lay<DP, MODE>::NT)) chunk_kernel(const ChunkArgs g) {
+    using L = Lay<DP, MODE>;
+    constexpr int NW = L::NW, RS = L::RS, G = DP / 32;
+    constexpr bool BWD = MODE == TWO || MODE == THREE;
+    extern __shared__ __align__(16) char lds[];
+    Powers& pw = *(Powers*)lds;
+    T* const rows0 = (T*)(lds + sizeof(Powers));
+    T* const turn0 = rows0 + L::NROWS * L::ROWS;
+    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), grp = wave / NW, wv = wave % NW;
+    const long heads = (long)g.B * g.J * g.H;
+    const int bid = xcd_remap(blockIdx.x, gridDim.x), seg = (int)(bid / heads);
+    const long hd = bid - seg * heads;
+    const int h = (int)(hd % g.H), j = (int)(hd / g.H % g.J);
+    const long b = hd / g.H / g.J;
+    const Role& ro = g.role[BWD ? grp : 0];
+    const bool rev = ro.reverse;
+    const int len = g.lengths ? min(max(g.lengths[b], 0), g.T) : g.T;
+    const int s0 = seg * g.L, s1 = min(s0 + g.L, g.T), e1 = min(s1, len), count = max(e1 - s0, 0);     // tokens [s0, e1), padding behind them
+    const int nchunk = (count + CT - 1) / CT;
+    if (MODE == SUMS && (!count || (g.skip_last && (rev ? s0 == 0 : e1 == len)))) return;
+    if (tid <= CT) {
+        const double x = (double)g.log_decay[h] * tid;     // (64 bits: a head that remembers n tokens adds up n such errors)
+        pw.p[tid] = tid ? (float)exp(x) : 1.f;             // (minus infinity: lambda^0 is 1 all the same)
+        pw.m[tid] = tid ? (float)expm1(x) : 0.f;
+    }
+    // ---- roles: dv (a, b, c) = (k, q, do), dk (v, do, q), dq (do, v, k); turned tiles of BWD: q, do (, k)
+    const int ia = BWD ? (grp == 0 ? 2 : grp == 1 ? 3 : 1) : 0, ib = BWD ? (grp == 0 ? 0 : grp == 1 ? 1 : 3) : 1, ic = BWD ? (grp == 0 ? 1 : grp == 1 ? 0 : 2) : 2;
+    const T *ta = rows0 + ia * L::ROWS, *tb = rows0 + ib * L::ROWS;
+    const T *tbT = turn0 + (BWD ? ib : 0) * L::TURN;
+    T* const tc = turn0 + (BWD ? ic : 1) * L::TURN + wv * 32 * TS;                 // this wave's 32 columns of c
+    T* const to = BWD ? turn0 + L::NTURN * L::TURN + wave * 32 * TS : tc;
+    const bool states = MODE != THREE || grp < 2;
+    const int c0 = wv * 32 + col, D1 = ro.D1, D2 = ro.D2;
+
+    f32x16 X[G];
+    {
+        const float* xin = MODE != SUMS && ro.xin ? ro.xin + (hd * g.nseg + seg) * (long)(D1 * D2) : nullptr;
+#pragma unroll
+        for (int q = 0; q < G; ++q)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int d = 32 * q + 8 * (r >> 2) + 4 * half + (r & 3);
+                X[q][r] = xin && d < D1 && c0 < D2 ? xin[ro.turn ? c0 * D1 + d : d * D2 + c0] : 0.f;
+            }
+    }
+    // ---- which tensors this group of waves brings in: ONE and SUMS all, TWO (q, k) and (do, v), THREE (q, v), do, k
+    constexpr int NS = MODE == ONE ? 3 : 2;
+    const int st[3] = {MODE == ONE ? 0 : MODE == SUMS ? 1 : grp, MODE == ONE ? 1 : MODE == SUMS ? 2 : MODE == TWO ? 2 + grp : grp ? -1 : 3, 2};
+    View in[NS];
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+        const int k = max(st[i], 0);
+        in[i] = View{(const T*)g.in[k].p + seq_at(g.in[k], b, 0, j, h), g.in[k].t, g.D[k], g.al[k]};
+    }
+    Stage<T> stage[NS];
+    auto fetch = [&](int c) {
+        const int t0 = s0 + c * CT, n = min(CT, e1 - t0);
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+            if (st[i] >= 0) stage[i].load(in[i], t0, n, wv, lane);
+    };
+    auto place = [&]() {
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+            if (st[i] < 0) continue;
+            if (MODE == ONE ? i < 2 : MODE != SUMS) stage[i].template rows<RS>(rows0 + st[i] * L::ROWS, wv, lane);
+            if (MODE == ONE ? i > 0 : MODE == SUMS || st[i] < L::NTURN) stage[i].turned(turn0 + (BWD ? st[i] : st[i] - 1) * L::TURN, wv, lane);
+        }
+    };
+    if (nchunk) {
+        fetch(rev && MODE != THREE ? nchunk - 1 : 0);
+        place();
+    }
+    __syncthreads();
+    // powers that every chunk uses: lambda^|i - j| of the scores this lane holds, for tokens j = 8 (r / 4) + 4 half + r % 4 and i = col
+    float pd[16];
+    if constexpr (MODE != SUMS)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int k = 8 * (r >> 2) + 4 * half + (r & 3), gap = rev ? k - col : col - k;
+            pd[r] = gap >= 0 ? pw.p[gap] * ro.fp : 0.f;
+        }
+    T* const O = (T*)ro.out.p + (MODE == SUMS ? 0 : seq_at(ro.out, b, 0, j, h));
+    for (int c = 0; c < nchunk; ++c) {
+        const int ch = rev ? nchunk - 1 - c : c, t0 = s0 + ch * CT, n = min(CT, e1 - t0);
+        if (c + 1 < nchunk) fetch(rev ? ch - 1 : ch + 1);
+        // backward in time the gradient of the last state meets the last token undecayed
+        const int first = rev && t0 + n == len ? 1 : 0;
+        f32x16 Y = {};
+        float p[16];
+        if constexpr (MODE != SUMS) {
+            f32x16 P = {};
+#pragma unroll
+            for (int q = 0; q < G; ++q) {
+                const Frag<T> fa = ld_frag(ta + col * RS + 32 * q, half), fb = ld_frag(tb + col * RS + 32 * q, half);
+                mma(P, fb, fa);                            // P[j][i] = b_j a_i
+                mma_fs(Y, X[q], fa);                       // Y[e][i] = sum_d X[d][e] a_i[d]
+            }
+            const float od = pw.p[max((rev ? n - 1 - col : col) + 1 - first, 0)] * ro.fo;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int k = 8 * (r >> 2) + 4 * half + (r & 3);
+                p[r] = (rev ? k >= col : k <= col) ? P[r] * pd[r] : 0.f;
+                Y[r] *= od;
+            }
+        }
+        const Frag<T> fc = ld_frag(tc + col * TS, half);
+        if constexpr (MODE != SUMS) {
+            Prepared<T> pp;
+            pp.set(p);
+            mma_sf(Y, fc, pp.v);                           // Y[e][i] += sum_j c_j[e] P[j][i]
+        }
+        if (states) {
+            float v[16];
+            unpack(fc, v);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int k = 8 * (r >> 2) + 4 * half + (r & 3);
+                v[r] *= pw.p[rev ? k : max(n - 1 - k, 0)] * ro.fk;
+            }
+            Exact<T> pv;
+            pv.set(v);
+            // lambda^m X as X + (lambda^m - 1) X where that is the more exact of the two
+            const int m = n - first;
+            const bool near = pw.p[m] >= 0.5f;
+            const float xm = near ? pw.m[m] : pw.p[m], one = near ? 1.f : 0.f;
+#pragma unroll
+            for (int q = 0; q < G; ++q) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) X[q][r] = fmaf(X[q][r], xm, one * X[q][r]);
+                mma_sf(X[q], ld_frag(tbT + (32 * q + col) * TS, half), pv.v);
+            }
+        }
+        if constexpr (MODE != SUMS) put_tile<T>(Y, to, O, ro.out.t, t0, n, wv * 32, D2, ro.al, lane);
+        __syncthreads();
+        if (c + 1 < nchunk) {
+            place();
+            __syncthreads();
+        }
+    }
+    if (MODE != SUMS && s1 > max(e1, s0)) put_zeros<T>(O, ro.out.t, max(e1, s0), s1, D2, ro.al, tid - grp * NW * 64, NW * 64);
+    if (ro.xout && states) {
+        float* xo = ro.xout + (hd * g.nseg + seg) * (long)(D1 * D2);
+        const float f = MODE != SUMS && rev && len ? pw.p[1] : 1.f;
+#pragma unroll
+        for (int q = 0; q < G; ++q)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int d = 32 * q + 8 * (r >> 2) + 4 * half + (r & 3);
+                if (d < D1 && c0 < D2) xo[d * D2 + c0] = X[q][r] * f;
+            }
+    }
+}
+
+// The states before every segment (in place of the segments' sums) and behind the last: one thread an element, segment by segment.
+struct JoinArgs {
+    float* ws;                       // [head][segment][D1 D2]
+    const float* first;              // [head][D1 D2], the state before the first segment in this direction, or null
+    float* last;
+    const float* log_decay;
+    const int32_t* lengths;
+    int T, J, H, nseg, L, size, reverse;
+};
+__global__ void __launch_bounds__(256) join_kernel(const JoinArgs g) {
+    const long hd = blockIdx.x;
+    const int i = blockIdx.y * 256 + threadIdx.x;
+    const int h = (int)(hd % g.H);
+    const long b = hd / g.H / g.J;
+    const int len = g.lengths ? min(max(g.lengths[b], 0), g.T) : g.T;
+    if (i >= g.size) return;
+    const double lg = g.log_decay[h];
+    const int n = (len + g.L - 1) / g.L;                   // segments that hold tokens
+    float x = g.first ? g.first[hd * g.size + i] : 0.f;
+    float* w = g.ws + hd * g.nseg * g.size + i;
+    const float whole = (float)exp(lg * g.L);
+#pragma unroll 4
+    for (int k = 0; k < n; ++k) {
+        const int s = g.reverse ? n - 1 - k : k, count = min(g.L, len - s * g.L), m = count - (g.reverse && k == 0 ? 1 : 0);
+        const float f = m == g.L ? whole : m ? (float)exp(lg * m) : 1.f;
+        float* at = w + (long)s * g.size;
+        const bool sums = g.last || k + 1 < n;             // (the last segment's sums are only there where somebody wants the last state)
+        const float e = sums ? *at : 0.f;
+        *at = x;
+        x = fmaf(f, x, e);
+    }
+    if (g.last) g.last[hd * g.size + i] = g.reverse && len ? (float)exp(lg) * x : x;
 }
 
 // One token: a block per head, the state is read and written once (that is the whole cost: 8 Dk Dv bytes), VE columns a thread, the rows
@@ -155,53 +584,160 @@ int check(const gast_decay_args* p) {
     if (!p || p->B < 1 || p->T < 1 || p->J < 1 || p->H < 1 || p->Dk < 1 || p->Dv < 1 || !p->log_decay) return GAST_EINVAL;
     if (p->dtype != GAST_F32 && p->dtype != GAST_BF16) return GAST_EINVAL;
     if (!p->q.p || !p->k.p || !p->v.p) return GAST_EINVAL;
-    if (p->Dk > GAST_DECAY_MAX_D || p->Dv > GAST_DECAY_MAX_D) return GAST_ERANGE;
+    if (p->Dk > GAST_DECAY_MAX_D || p->Dv > GAST_DECAY_MAX_D || p->T > (1 << 30)) return GAST_ERANGE;
     return 0;
 }
 
-ScanArgs roles(const gast_decay_args& g, const gast_seq& a, const gast_seq& b, const gast_seq& c, const gast_seq& out, int D1, int D2) {
-    ScanArgs p = {};
-    p.a = a; p.b = b; p.c = c; p.out = out; p.D1 = D1; p.D2 = D2;
-    p.log_decay = g.log_decay; p.lengths = g.lengths; p.B = g.B; p.T = g.T; p.J = g.J; p.H = g.H;
-    p.bscale = p.oscale = 1.f;
-    return p;
+// How the tokens are cut: one segment where the heads alone fill the card (two waves for each of its 1024 SIMDs), else as many as that
+// takes, of at least 256 tokens: a cut costs a second reading of two of the tensors and a state for each segment and head.
+struct Cut { int dp, nseg, L; };
+Cut cut(long heads, int T, int Dk, int Dv) {
+    const int D = Dk > Dv ? Dk : Dv;
+    Cut c;
+    c.dp = D <= 32 ? 32 : D <= 64 ? 64 : 128;
+    const long want = (2048 * 32 / c.dp + heads - 1) / heads, most = T / 256;
+    const long n = want < most ? want : most;
+    c.nseg = n < 2 ? 1 : (int)n;
+    c.L = ((T + c.nseg - 1) / c.nseg + CT - 1) / CT * CT;
+    c.nseg = (T + c.L - 1) / c.L;
+    return c;
+}
+
+template <typename T, int DP, int MODE>
+int launch(const ChunkArgs& g, hipStream_t s) {
+    using L = Lay<DP, MODE>;
+    constexpr int bytes = (int)sizeof(Powers) + L::ELEMS * (int)sizeof(T);
+    const long blocks = (long)g.B * g.J * g.H * g.nseg;
+    if (blocks > 0x7fffffffL) return GAST_ERANGE;
+    static_assert(bytes <= 160 * 1024, "LDS of a CU");
+    if (bytes > 64 * 1024) {
+        static std::atomic<bool> done[64];
+        int dev = 0;
+        if (hipError_t e = hipGetDevice(&dev)) return (int)e;
+        if (dev >= 64 || !done[dev].load(std::memory_order_acquire)) {       // (an attribute of the device; a racing first call repeats it)
+            if (hipError_t e = hipFuncSetAttribute((const void*)chunk_kernel<T, DP, MODE>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes)) return (int)e;
+            if (dev < 64) done[dev].store(true, std::memory_order_release);
+        }
+    }
+    hipLaunchKernelGGL((chunk_kernel<T, DP, MODE>), dim3((unsigned)blocks), dim3(L::NT), bytes, s, g);
+    GAST_CHECK_LAUNCH();
+    return 0;
+}
+template <typename T, int MODE>
+int launch_dp(const ChunkArgs& g, int dp, hipStream_t s) {
+    if (dp == 32) return launch<T, 32, MODE>(g, s);
+    if (dp == 64) return launch<T, 64, MODE>(g, s);
+    if constexpr (MODE != THREE) return launch<T, 128, MODE>(g, s);
+    return GAST_EINVAL;
+}
+
+ChunkArgs chunk_args(const gast_decay_args& g, const Cut& c) {
+    ChunkArgs a = {};
+    a.log_decay = g.log_decay; a.lengths = g.lengths; a.B = g.B; a.T = g.T; a.J = g.J; a.H = g.H; a.nseg = c.nseg; a.L = c.L;
+    return a;
+}
+int on16(const gast_seq& s, int dtype) { return seq_align(s, dtype == GAST_F32 ? 4 : 2, dtype == GAST_F32 ? 4 : 8) == (dtype == GAST_F32 ? 4 : 8); }
+void put_in(ChunkArgs& a, int i, const gast_seq& s, int D, int dtype) { a.in[i] = s; a.D[i] = D; a.al[i] = on16(s, dtype); }
+Role role_of(const gast_seq& out, int D1, int D2, int reverse, float scale, int dtype) {
+    Role r = {};
+    r.out = out; r.D1 = D1; r.D2 = D2; r.al = out.p ? on16(out, dtype) : 0; r.reverse = reverse;
+    r.fp = scale; r.fk = reverse ? scale : 1.f; r.fo = reverse ? 1.f : scale;
+    return r;
+}
+
+// sums of the segments of b c' and the states between them, into ws
+template <typename T>
+int states(const gast_decay_args& g, const Cut& c, const gast_seq& b, const gast_seq& cc, int reverse, const float* first, float* last, float* ws, hipStream_t s) {
+    ChunkArgs a = chunk_args(g, c);
+    put_in(a, 1, b, g.Dk, g.dtype);
+    put_in(a, 2, cc, g.Dv, g.dtype);
+    a.role[0] = role_of(gast_seq{}, g.Dk, g.Dv, reverse, g.scale, g.dtype);
+    a.role[0].xout = ws;
+    a.skip_last = !last;
+    if (int rc = launch_dp<T, SUMS>(a, c.dp, s)) return rc;
+    JoinArgs j = {ws, first, last, g.log_decay, g.lengths, g.T, g.J, g.H, c.nseg, c.L, g.Dk * g.Dv, reverse};
+    hipLaunchKernelGGL(join_kernel, dim3((unsigned)((long)g.B * g.J * g.H), (unsigned)((j.size + 255) / 256)), dim3(256), 0, s, j);
+    GAST_CHECK_LAUNCH();
+    return 0;
 }
 
 template <typename T>
 int forward(const gast_decay_args& g, hipStream_t s) {
-    ScanArgs p = roles(g, g.q, g.k, g.v, g.o, g.Dk, g.Dv);
-    p.xin = g.state; p.xout = g.state_out; p.oscale = g.scale;
-    return scan<T>(p, s);
+    const Cut c = cut((long)g.B * g.J * g.H, g.T, g.Dk, g.Dv);
+    ChunkArgs a = chunk_args(g, c);
+    put_in(a, 0, g.q, g.Dk, g.dtype);
+    put_in(a, 1, g.k, g.Dk, g.dtype);
+    put_in(a, 2, g.v, g.Dv, g.dtype);
+    a.role[0] = role_of(g.o, g.Dk, g.Dv, 0, g.scale, g.dtype);
+    if (c.nseg > 1) {
+        if (int rc = states<T>(g, c, g.k, g.v, 0, g.state, g.state_out, g.ws, s)) return rc;
+        a.role[0].xin = g.ws;
+    } else {
+        a.role[0].xin = g.state;
+        a.role[0].xout = g.state_out;
+    }
+    return launch_dp<T, ONE>(a, c.dp, s);
 }
 
 template <typename T>
 int backward(const gast_decay_args& g, hipStream_t s) {
-    ScanArgs p = roles(g, g.d_o, g.v, g.k, g.dq, g.Dv, g.Dk);
-    p.xin = g.state; p.xin_t = 1; p.oscale = g.scale;
-    if (int rc = scan<T>(p, s)) return rc;
-    p = roles(g, g.k, g.q, g.d_o, g.dv, g.Dk, g.Dv);
-    p.reverse = 1; p.xin = g.dstate_out; p.xout = g.dstate; p.bscale = g.scale;
-    if (int rc = scan<T>(p, s)) return rc;
-    p = roles(g, g.v, g.d_o, g.q, g.dk, g.Dv, g.Dk);
-    p.reverse = 1; p.xin = g.dstate_out; p.xin_t = 1; p.bscale = g.scale;
-    return scan<T>(p, s);
+    const Cut c = cut((long)g.B * g.J * g.H, g.T, g.Dk, g.Dv);
+    const long size = (long)g.B * g.J * g.H * c.nseg * g.Dk * g.Dv;
+    const float *before = g.state, *behind = g.dstate_out;
+    if (c.nseg > 1) {
+        if (int rc = states<T>(g, c, g.k, g.v, 0, g.state, nullptr, g.ws, s)) return rc;
+        if (int rc = states<T>(g, c, g.q, g.d_o, 1, g.dstate_out, g.dstate, g.ws + size, s)) return rc;
+        before = g.ws;
+        behind = g.ws + size;
+    }
+    ChunkArgs a = chunk_args(g, c);
+    put_in(a, 0, g.q, g.Dk, g.dtype);
+    put_in(a, 1, g.d_o, g.Dv, g.dtype);
+    put_in(a, 2, g.k, g.Dk, g.dtype);
+    put_in(a, 3, g.v, g.Dv, g.dtype);
+    a.role[0] = role_of(g.dv, g.Dk, g.Dv, 1, g.scale, g.dtype);
+    a.role[0].xin = behind;
+    a.role[0].xout = c.nseg > 1 ? nullptr : g.dstate;
+    a.role[1] = role_of(g.dk, g.Dv, g.Dk, 1, g.scale, g.dtype);
+    a.role[1].xin = behind;
+    a.role[1].turn = 1;
+    Role dq = role_of(g.dq, g.Dv, g.Dk, 0, g.scale, g.dtype);
+    dq.xin = before;
+    dq.turn = 1;
+    if (g.T <= CT && c.dp <= 64) {
+        a.role[2] = dq;
+        return launch_dp<T, THREE>(a, c.dp, s);
+    }
+    if (int rc = launch_dp<T, TWO>(a, c.dp, s)) return rc;
+    ChunkArgs d = chunk_args(g, c);
+    put_in(d, 0, g.d_o, g.Dv, g.dtype);
+    put_in(d, 1, g.v, g.Dv, g.dtype);
+    put_in(d, 2, g.k, g.Dk, g.dtype);
+    d.role[0] = dq;
+    return launch_dp<T, ONE>(d, c.dp, s);
 }
 
 }  // namespace
 
 extern "C" int gast_decay_fwd(const gast_decay_args* args, gast_stream_t stream) {
     if (int rc = check(args)) return rc;
-    if (!args->o.p) return GAST_EINVAL;
+    if (!args->o.p || (!args->ws && gast_decay_ws_floats(args->B, args->T, args->J, args->H, args->Dk, args->Dv, 0))) return GAST_EINVAL;
     return args->dtype == GAST_F32 ? forward<float>(*args, (hipStream_t)stream) : forward<bf16_t>(*args, (hipStream_t)stream);
 }
 
 extern "C" int gast_decay_bwd(const gast_decay_args* args, gast_stream_t stream) {
     if (int rc = check(args)) return rc;
     if (!args->d_o.p || !args->dq.p || !args->dk.p || !args->dv.p) return GAST_EINVAL;
+    if (!args->ws && gast_decay_ws_floats(args->B, args->T, args->J, args->H, args->Dk, args->Dv, 1)) return GAST_EINVAL;
     return args->dtype == GAST_F32 ? backward<float>(*args, (hipStream_t)stream) : backward<bf16_t>(*args, (hipStream_t)stream);
 }
 
-extern "C" long gast_decay_ws_floats(int B, int T, int J, int H, int Dk, int Dv, int backward) { return 0; }
+extern "C" long gast_decay_ws_floats(int B, int T, int J, int H, int Dk, int Dv, int backward) {
+    const long heads = (long)B * J * H;
+    if (heads < 1 || T < 1) return 0;
+    const Cut c = cut(heads, T, Dk, Dv);
+    return c.nseg > 1 ? heads * c.nseg * Dk * Dv * (backward ? 2 : 1) : 0;
+}
 
 extern "C" int gast_decay_step(const gast_decay_args* args, gast_stream_t stream) {
     if (int rc = check(args)) return rc;
