@@ -190,29 +190,19 @@ template <> struct Exact<bf16_t> { Parts v; __device__ __forceinline__ void set(
 
 // The 32 x DP tokens of one tensor on their way from memory to LDS: 16 elements a thread of NW waves.  16 bits: 8 channels of two rows,
 // so that a turned word holds both; four lanes read 64 contiguous bytes and the turned words of a wave fall into 64 different banks.
-struct View { const void* p; long t; int D, al; };       // token 0 of the sequence, its stride, channels, 16-byte rows
+struct View { const void* p; long t; int D; };           // token 0 of the sequence, its stride, channels
 template <typename T> struct Stage;
 template <> struct Stage<bf16_t> {
-    uint4 x[2];
-    __device__ __forceinline__ void load(const View& s, int t0, int n, int wv, int lane) {
-        const int d = (wv * 4 + (lane & 3)) * 8, row = (lane >> 2) * 2;
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            x[k] = make_uint4(0, 0, 0, 0);
-            if (row + k >= n || d >= s.D) continue;
-            const bf16_t* p = (const bf16_t*)s.p + (long)(t0 + row + k) * s.t + d;
-            if (s.al && d + 8 <= s.D) {
-                x[k] = *(const uint4*)p;
-            } else {
-                uint32_t w[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    w[e] = d + 2 * e < s.D ? p[2 * e] : 0;
-                    if (d + 2 * e + 1 < s.D) w[e] |= (uint32_t)p[2 * e + 1] << 16;
-                }
-                x[k] = make_uint4(w[0], w[1], w[2], w[3]);
-            }
-        }
+    static constexpr int NV = 2;
+    uint4 x[NV];
+    static __device__ __forceinline__ int row(int lane, int k) { return (lane >> 2) * 2 + k; }
+    static __device__ __forceinline__ int chan(int wv, int lane, int) { return (wv * 4 + (lane & 3)) * 8; }
+    __device__ __forceinline__ void none(int k) { x[k] = make_uint4(0, 0, 0, 0); }
+    __device__ __forceinline__ void vec(int k, const char* p) { x[k] = *(const uint4*)p; }
+    __device__ __forceinline__ void some(int k, const bf16_t* p, int n) {
+        uint32_t w[4] = {0, 0, 0, 0};
+        for (int e = 0; e < 8 && e < n; ++e) w[e >> 1] |= (uint32_t)p[e] << 16 * (e & 1);
+        x[k] = make_uint4(w[0], w[1], w[2], w[3]);
     }
     template <int RS> __device__ __forceinline__ void rows(bf16_t* tile, int wv, int lane) const {
         bf16_t* p = tile + (lane >> 2) * 2 * RS + (wv * 4 + (lane & 3)) * 8;
@@ -233,37 +223,55 @@ template <> struct Stage<bf16_t> {
     }
 };
 template <> struct Stage<float> {
-    float4 x[4];
-    __device__ __forceinline__ void load(const View& s, int t0, int n, int wv, int lane) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int d = (wv * 8 + (lane & 3) + 4 * (k & 1)) * 4, row = (lane >> 2) + 16 * (k >> 1);
-            x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (row >= n || d >= s.D) continue;
-            const float* p = (const float*)s.p + (long)(t0 + row) * s.t + d;
-            if (s.al && d + 4 <= s.D) {
-                x[k] = *(const float4*)p;
-            } else {
-                x[k].x = p[0];
-                if (d + 1 < s.D) x[k].y = p[1];
-                if (d + 2 < s.D) x[k].z = p[2];
-                if (d + 3 < s.D) x[k].w = p[3];
-            }
-        }
+    static constexpr int NV = 4;
+    float4 x[NV];
+    static __device__ __forceinline__ int row(int lane, int k) { return (lane >> 2) + 16 * (k >> 1); }
+    static __device__ __forceinline__ int chan(int wv, int lane, int k) { return (wv * 8 + (lane & 3) + 4 * (k & 1)) * 4; }
+    __device__ __forceinline__ void none(int k) { x[k] = make_float4(0.f, 0.f, 0.f, 0.f); }
+    __device__ __forceinline__ void vec(int k, const char* p) { x[k] = *(const float4*)p; }
+    __device__ __forceinline__ void some(int k, const float* p, int n) {
+        x[k] = make_float4(p[0], n > 1 ? p[1] : 0.f, n > 2 ? p[2] : 0.f, n > 3 ? p[3] : 0.f);
     }
     template <int RS> __device__ __forceinline__ void rows(float* tile, int wv, int lane) const {
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-            *(float4*)(tile + ((lane >> 2) + 16 * (k >> 1)) * RS + (wv * 8 + (lane & 3) + 4 * (k & 1)) * 4) = x[k];
+        for (int k = 0; k < 4; ++k) *(float4*)(tile + row(lane, k) * RS + chan(wv, lane, k)) = x[k];
     }
     __device__ __forceinline__ void turned(float* tile, int wv, int lane) const {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            float* p = tile + (wv * 8 + (lane & 3) + 4 * (k & 1)) * 4 * TS + (lane >> 2) + 16 * (k >> 1);
+            float* p = tile + chan(wv, lane, k) * TS + row(lane, k);
             p[0] = x[k].x; p[TS] = x[k].y; p[2 * TS] = x[k].z; p[3 * TS] = x[k].w;
         }
     }
 };
+// The loads of a chunk are issued while the one before is worked on, so they stand in straight code (a join of two paths would wait for
+// them): every lane reads a whole vector at a block-uniform base plus a 32-bit offset, at a row and channel that exist, and what is behind
+// the chunk's end or the head's last channel becomes zero on the way to LDS.
+template <typename T>
+__device__ __forceinline__ void bring(Stage<T>& s, const View& v, int t0, int n, int wv, int lane) {
+    const char* base = (const char*)v.p + (long)t0 * v.t * (int)sizeof(T);
+#pragma unroll
+    for (int k = 0; k < Stage<T>::NV; ++k) {
+        const int d = Stage<T>::chan(wv, lane, k), row = min(Stage<T>::row(lane, k), n - 1);
+        s.vec(k, base + (uint32_t)(row * (int)v.t + (d < v.D ? d : 0)) * (uint32_t)sizeof(T));
+    }
+}
+template <typename T>
+__device__ __forceinline__ void trim(Stage<T>& s, const View& v, int n, int wv, int lane) {
+#pragma unroll
+    for (int k = 0; k < Stage<T>::NV; ++k)
+        if (Stage<T>::row(lane, k) >= n || Stage<T>::chan(wv, lane, k) >= v.D) s.none(k);
+}
+// rows that do not start on 16 bytes, or heads that do not end there: element by element, not ahead of time
+template <typename T>
+__device__ __forceinline__ void bring_odd(Stage<T>& s, const View& v, int t0, int n, int wv, int lane) {
+#pragma unroll
+    for (int k = 0; k < Stage<T>::NV; ++k) {
+        const int d = Stage<T>::chan(wv, lane, k), row = Stage<T>::row(lane, k);
+        s.none(k);
+        if (row < n && d < v.D) s.some(k, (const T*)v.p + (long)(t0 + row) * v.t + d, v.D - d);
+    }
+}
 
 // Y (32 columns of out by 32 tokens, the token in lane % 32) to memory by way of LDS, so that a row leaves in 16-byte pieces
 template <typename T>
@@ -337,10 +345,18 @@ template <int DP, int MODE> struct Lay {
     static constexpr int ELEMS = NROWS * ROWS + NTURN * TURN + OUT;
 };
 
-struct Powers { float p[CT + 4], m[CT + 4]; };            // lambda^n, and lambda^n - 1
+// exp(g n) to two steps of fp32, however long n is: the product's rounding is carried along
+__device__ __forceinline__ float power(float g, float n) {
+    if (n == 0.f) return 1.f;                              // (minus infinity: lambda^0 is 1 all the same)
+    const float x = g * n, rest = fmaf(g, n, -x), e = expf(x);
+    return e > 0.f && e < INFINITY ? fmaf(e, rest, e) : e;
+}
+struct Powers { float up[CT + 4], down[CT + 4]; };        // lambda^k, k = 0 .. 32; down[k] = lambda^(31 - k)
 
-template <typename T, int DP, int MODE>
-__global__ void __launch_bounds__((Lay<DP, MODE>::NT)) chunk_kernel(const ChunkArgs g) {
+// The state is held as X = acc * Xh with acc = lambda^(tokens since it was last brought up to date): decaying the accumulators costs nothing
+// until acc leaves [2^-8, 2^8].  What enters is divided by acc, what leaves multiplied.
+template <typename T, int DP, int MODE, bool VEC>
+__global__ void __launch_bounds__((Lay<DP, MODE>::NT), 2) chunk_kernel(const ChunkArgs g) {
     using L = Lay<DP, MODE>;
     constexpr int NW = L::NW, RS = L::RS, G = DP / 32;
     constexpr bool BWD = MODE == TWO || MODE == THREE;
@@ -350,147 +366,171 @@ __global__ void __launch_bounds__((Lay<DP, MODE>::NT)) chunk_kernel(const ChunkA
     T* const turn0 = rows0 + L::NROWS * L::ROWS;
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), grp = wave / NW, wv = wave % NW;
-    const long heads = (long)g.B * g.J * g.H;
-    const int bid = xcd_remap(blockIdx.x, gridDim.x), seg = (int)(bid / heads);
-    const long hd = bid - seg * heads;
-    const int h = (int)(hd % g.H), j = (int)(hd / g.H % g.J);
-    const long b = hd / g.H / g.J;
+    const uint32_t heads = (uint32_t)g.B * g.J * g.H, bid = xcd_remap(blockIdx.x, gridDim.x);
+    const uint32_t seg = g.nseg > 1 ? bid / heads : 0, hd = bid - seg * heads, bj = hd / (uint32_t)g.H, h = hd - bj * g.H, b = bj / (uint32_t)g.J, j = bj - b * g.J;
     const Role& ro = g.role[BWD ? grp : 0];
-    const bool rev = ro.reverse;
+    const bool rev = MODE == ONE ? false : MODE == TWO ? true : MODE == THREE ? grp < 2 : ro.reverse;
     const int len = g.lengths ? min(max(g.lengths[b], 0), g.T) : g.T;
-    const int s0 = seg * g.L, s1 = min(s0 + g.L, g.T), e1 = min(s1, len), count = max(e1 - s0, 0);     // tokens [s0, e1), padding behind them
+    const int s0 = (int)seg * g.L, s1 = min(s0 + g.L, g.T), e1 = min(s1, len), count = max(e1 - s0, 0);     // tokens [s0, e1), padding behind them
     const int nchunk = (count + CT - 1) / CT;
     if (MODE == SUMS && (!count || (g.skip_last && (rev ? s0 == 0 : e1 == len)))) return;
-    if (tid <= CT) {
-        const double x = (double)g.log_decay[h] * tid;     // (64 bits: a head that remembers n tokens adds up n such errors)
-        pw.p[tid] = tid ? (float)exp(x) : 1.f;             // (minus infinity: lambda^0 is 1 all the same)
-        pw.m[tid] = tid ? (float)expm1(x) : 0.f;
-    }
+    const float lg = g.log_decay[h];
     // ---- roles: dv (a, b, c) = (k, q, do), dk (v, do, q), dq (do, v, k); turned tiles of BWD: q, do (, k)
     const int ia = BWD ? (grp == 0 ? 2 : grp == 1 ? 3 : 1) : 0, ib = BWD ? (grp == 0 ? 0 : grp == 1 ? 1 : 3) : 1, ic = BWD ? (grp == 0 ? 1 : grp == 1 ? 0 : 2) : 2;
     const T *ta = rows0 + ia * L::ROWS, *tb = rows0 + ib * L::ROWS;
     const T *tbT = turn0 + (BWD ? ib : 0) * L::TURN;
     T* const tc = turn0 + (BWD ? ic : 1) * L::TURN + wv * 32 * TS;                 // this wave's 32 columns of c
     T* const to = BWD ? turn0 + L::NTURN * L::TURN + wave * 32 * TS : tc;
-    const bool states = MODE != THREE || grp < 2;
     const int c0 = wv * 32 + col, D1 = ro.D1, D2 = ro.D2;
+    const bool works = wv * 32 < D2;
 
+    // ---- which tensors this group of waves brings in: ONE and SUMS all, TWO (q, k) and (do, v), THREE (q, v), do, k
+    constexpr int NS = MODE == ONE ? 3 : 2;
+    const int st[3] = {MODE == ONE ? 0 : MODE == SUMS ? 1 : grp, MODE == ONE ? 1 : MODE == SUMS ? 2 : MODE == TWO ? 2 + grp : grp ? -1 : 3, 2};
+    View in[NS];
+    Stage<T> stage[NS];
+    bool whole = true;
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+        const int k = max(st[i], 0);
+        in[i] = View{(const T*)g.in[k].p + seq_at(g.in[k], b, 0, j, h), g.in[k].t, g.D[k]};
+        whole = whole && g.D[k] == DP;
+    }
+    auto fetch = [&](int c) {
+        const int t0 = s0 + c * CT, n = min(CT, e1 - t0);
+        if constexpr (VEC)
+#pragma unroll
+            for (int i = 0; i < NS; ++i) bring<T>(stage[i], in[i], t0, n, wv, lane);      // (THREE: two groups bring in nothing new the second time)
+    };
+    auto place = [&](int c) {
+        const int t0 = s0 + c * CT, n = min(CT, e1 - t0);
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+            if (st[i] < 0) continue;
+            if constexpr (VEC) { if (!whole || n < CT) trim<T>(stage[i], in[i], n, wv, lane); }
+            else bring_odd<T>(stage[i], in[i], t0, n, wv, lane);
+            if (MODE == ONE ? i < 2 : MODE != SUMS) stage[i].template rows<RS>(rows0 + st[i] * L::ROWS, wv, lane);
+            if (MODE == ONE ? i > 0 : MODE == SUMS || st[i] < L::NTURN) stage[i].turned(turn0 + (BWD ? st[i] : st[i] - 1) * L::TURN, wv, lane);
+        }
+    };
+    const int c_first = rev && MODE != THREE ? nchunk - 1 : 0;
+    if (nchunk) fetch(c_first);
+    if (tid <= CT) {
+        const float p = power(lg, (float)tid);
+        pw.up[tid] = p;
+        if (tid < CT) pw.down[CT - 1 - tid] = p;
+    }
     f32x16 X[G];
-    {
-        const float* xin = MODE != SUMS && ro.xin ? ro.xin + (hd * g.nseg + seg) * (long)(D1 * D2) : nullptr;
+    float acc = 1.f;
+    int since = 0;
+#pragma unroll
+    for (int q = 0; q < G; ++q) X[q] = f32x16{};
+    if (MODE != SUMS && ro.xin && works) {
+        const float* xin = ro.xin + ((long)hd * g.nseg + seg) * (D1 * D2);
+        const int sd = ro.turn ? 1 : D2;
+        xin += min(c0, D2 - 1) * (ro.turn ? D1 : 1);       // (columns behind the last repeat it: nothing of theirs is stored)
 #pragma unroll
         for (int q = 0; q < G; ++q)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const int d = 32 * q + 8 * (r >> 2) + 4 * half + (r & 3);
-                X[q][r] = xin && d < D1 && c0 < D2 ? xin[ro.turn ? c0 * D1 + d : d * D2 + c0] : 0.f;
+                const float x = xin[min(d, D1 - 1) * sd];
+                X[q][r] = d < D1 ? x : 0.f;
             }
     }
-    // ---- which tensors this group of waves brings in: ONE and SUMS all, TWO (q, k) and (do, v), THREE (q, v), do, k
-    constexpr int NS = MODE == ONE ? 3 : 2;
-    const int st[3] = {MODE == ONE ? 0 : MODE == SUMS ? 1 : grp, MODE == ONE ? 1 : MODE == SUMS ? 2 : MODE == TWO ? 2 + grp : grp ? -1 : 3, 2};
-    View in[NS];
-#pragma unroll
-    for (int i = 0; i < NS; ++i) {
-        const int k = max(st[i], 0);
-        in[i] = View{(const T*)g.in[k].p + seq_at(g.in[k], b, 0, j, h), g.in[k].t, g.D[k], g.al[k]};
-    }
-    Stage<T> stage[NS];
-    auto fetch = [&](int c) {
-        const int t0 = s0 + c * CT, n = min(CT, e1 - t0);
-#pragma unroll
-        for (int i = 0; i < NS; ++i)
-            if (st[i] >= 0) stage[i].load(in[i], t0, n, wv, lane);
-    };
-    auto place = [&]() {
-#pragma unroll
-        for (int i = 0; i < NS; ++i) {
-            if (st[i] < 0) continue;
-            if (MODE == ONE ? i < 2 : MODE != SUMS) stage[i].template rows<RS>(rows0 + st[i] * L::ROWS, wv, lane);
-            if (MODE == ONE ? i > 0 : MODE == SUMS || st[i] < L::NTURN) stage[i].turned(turn0 + (BWD ? st[i] : st[i] - 1) * L::TURN, wv, lane);
-        }
-    };
-    if (nchunk) {
-        fetch(rev && MODE != THREE ? nchunk - 1 : 0);
-        place();
-    }
+    const bool carries = MODE == SUMS || (MODE == ONE ? ro.xin || nchunk > 1 : true);      // is there a state to meet a?
+    const bool wanted = MODE == SUMS || (ro.xout && (MODE != THREE || grp < 2));             // ... and is the last one wanted?
+    if (nchunk) place(c_first);
     __syncthreads();
     // powers that every chunk uses: lambda^|i - j| of the scores this lane holds, for tokens j = 8 (r / 4) + 4 half + r % 4 and i = col
     float pd[16];
+    const uint32_t seen = (rev ? ~0u << col : ~0u >> (31 - col)) >> (4 * half);      // bit 8 (r / 4) + r % 4: token j of register r counts for i
     if constexpr (MODE != SUMS)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             const int k = 8 * (r >> 2) + 4 * half + (r & 3), gap = rev ? k - col : col - k;
-            pd[r] = gap >= 0 ? pw.p[gap] * ro.fp : 0.f;
+            pd[r] = pw.up[abs(gap)] * ro.fp;               // (the others are masked)
         }
     T* const O = (T*)ro.out.p + (MODE == SUMS ? 0 : seq_at(ro.out, b, 0, j, h));
     for (int c = 0; c < nchunk; ++c) {
         const int ch = rev ? nchunk - 1 - c : c, t0 = s0 + ch * CT, n = min(CT, e1 - t0);
         if (c + 1 < nchunk) fetch(rev ? ch - 1 : ch + 1);
-        // backward in time the gradient of the last state meets the last token undecayed
-        const int first = rev && t0 + n == len ? 1 : 0;
-        f32x16 Y = {};
-        float p[16];
-        if constexpr (MODE != SUMS) {
-            f32x16 P = {};
+        if (works) {
+            // backward in time the gradient of the last state meets the last token undecayed
+            const int first = rev && t0 + n == len ? 1 : 0;
+            f32x16 Y = {};
+            float p[16];
+            if constexpr (MODE != SUMS) {
+                f32x16 P = {};
 #pragma unroll
-            for (int q = 0; q < G; ++q) {
-                const Frag<T> fa = ld_frag(ta + col * RS + 32 * q, half), fb = ld_frag(tb + col * RS + 32 * q, half);
-                mma(P, fb, fa);                            // P[j][i] = b_j a_i
-                mma_fs(Y, X[q], fa);                       // Y[e][i] = sum_d X[d][e] a_i[d]
-            }
-            const float od = pw.p[max((rev ? n - 1 - col : col) + 1 - first, 0)] * ro.fo;
+                for (int q = 0; q < G; ++q) {
+                    const Frag<T> fa = ld_frag(ta + col * RS + 32 * q, half), fb = ld_frag(tb + col * RS + 32 * q, half);
+                    mma(P, fb, fa);                            // P[j][i] = b_j a_i
+                    if (carries) mma_fs(Y, X[q], fa);          // Y[e][i] = sum_d X[d][e] a_i[d]
+                }
+                const float od = pw.up[max((rev ? n - 1 - col : col) + 1 - first, 0)] * ro.fo * acc;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int k = 8 * (r >> 2) + 4 * half + (r & 3);
-                p[r] = (rev ? k >= col : k <= col) ? P[r] * pd[r] : 0.f;
-                Y[r] *= od;
+                for (int r = 0; r < 16; ++r) {
+                    p[r] = seen >> (8 * (r >> 2) + (r & 3)) & 1 ? P[r] * pd[r] : 0.f;
+                    Y[r] *= od;
+                }
             }
+            const Frag<T> fc = ld_frag(tc + col * TS, half);
+            if constexpr (MODE != SUMS) {
+                Prepared<T> pp;
+                pp.set(p);
+                mma_sf(Y, fc, pp.v);                           // Y[e][i] += sum_j c_j[e] P[j][i]
+            }
+            if (wanted || c + 1 < nchunk) {
+                const int m = n - first;
+                since += m;
+                acc = power(lg, (float)since);
+                if (!(acc > 0x1p-8f && acc < 0x1p8f)) {
+#pragma unroll
+                    for (int q = 0; q < G; ++q)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) X[q][r] *= acc;
+                    acc = 1.f;
+                    since = 0;
+                }
+                float v[16];
+                unpack(fc, v);
+                const float in_acc = ro.fk / acc;
+                const float* kd = rev ? pw.up : pw.down;           // token k enters with lambda^k, or lambda^(n - 1 - k)
+                if (rev || n == CT) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const float4 f = *(const float4*)(kd + 8 * q + 4 * half);
+                        v[4 * q] *= f.x * in_acc; v[4 * q + 1] *= f.y * in_acc; v[4 * q + 2] *= f.z * in_acc; v[4 * q + 3] *= f.w * in_acc;
+                    }
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) v[r] *= pw.up[max(n - 1 - (8 * (r >> 2) + 4 * half + (r & 3)), 0)] * in_acc;
+                }
+                Exact<T> pv;
+                pv.set(v);
+#pragma unroll
+                for (int q = 0; q < G; ++q) mma_sf(X[q], ld_frag(tbT + (32 * q + col) * TS, half), pv.v);
+            }
+            if constexpr (MODE != SUMS) put_tile<T>(Y, to, O, ro.out.t, t0, n, wv * 32, D2, ro.al, lane);
         }
-        const Frag<T> fc = ld_frag(tc + col * TS, half);
-        if constexpr (MODE != SUMS) {
-            Prepared<T> pp;
-            pp.set(p);
-            mma_sf(Y, fc, pp.v);                           // Y[e][i] += sum_j c_j[e] P[j][i]
-        }
-        if (states) {
-            float v[16];
-            unpack(fc, v);
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int k = 8 * (r >> 2) + 4 * half + (r & 3);
-                v[r] *= pw.p[rev ? k : max(n - 1 - k, 0)] * ro.fk;
-            }
-            Exact<T> pv;
-            pv.set(v);
-            // lambda^m X as X + (lambda^m - 1) X where that is the more exact of the two
-            const int m = n - first;
-            const bool near = pw.p[m] >= 0.5f;
-            const float xm = near ? pw.m[m] : pw.p[m], one = near ? 1.f : 0.f;
-#pragma unroll
-            for (int q = 0; q < G; ++q) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) X[q][r] = fmaf(X[q][r], xm, one * X[q][r]);
-                mma_sf(X[q], ld_frag(tbT + (32 * q + col) * TS, half), pv.v);
-            }
-        }
-        if constexpr (MODE != SUMS) put_tile<T>(Y, to, O, ro.out.t, t0, n, wv * 32, D2, ro.al, lane);
-        __syncthreads();
         if (c + 1 < nchunk) {
-            place();
+            __syncthreads();
+            place(rev ? ch - 1 : ch + 1);
             __syncthreads();
         }
     }
     if (MODE != SUMS && s1 > max(e1, s0)) put_zeros<T>(O, ro.out.t, max(e1, s0), s1, D2, ro.al, tid - grp * NW * 64, NW * 64);
-    if (ro.xout && states) {
-        float* xo = ro.xout + (hd * g.nseg + seg) * (long)(D1 * D2);
-        const float f = MODE != SUMS && rev && len ? pw.p[1] : 1.f;
+    if (wanted && works) {
+        float* xo = ro.xout + ((long)hd * g.nseg + seg) * (D1 * D2);
+        const float f = MODE != SUMS && rev && len ? pw.up[1] * acc : acc;
+        if (c0 >= D2) return;
 #pragma unroll
         for (int q = 0; q < G; ++q)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const int d = 32 * q + 8 * (r >> 2) + 4 * half + (r & 3);
-                if (d < D1 && c0 < D2) xo[d * D2 + c0] = X[q][r] * f;
+                if (d < D1) xo[d * D2 + c0] = X[q][r] * f;
             }
     }
 }
@@ -594,7 +634,7 @@ struct Cut { int dp, nseg, L; };
 Cut cut(long heads, int T, int Dk, int Dv) {
     const int D = Dk > Dv ? Dk : Dv;
     Cut c;
-    c.dp = D <= 32 ? 32 : D <= 64 ? 64 : 128;
+    c.dp = (D + 31) / 32 * 32;
     const long want = (2048 * 32 / c.dp + heads - 1) / heads, most = T / 256;
     const long n = want < most ? want : most;
     c.nseg = n < 2 ? 1 : (int)n;
@@ -603,7 +643,7 @@ Cut cut(long heads, int T, int Dk, int Dv) {
     return c;
 }
 
-template <typename T, int DP, int MODE>
+template <typename T, int DP, int MODE, bool VEC>
 int launch(const ChunkArgs& g, hipStream_t s) {
     using L = Lay<DP, MODE>;
     constexpr int bytes = (int)sizeof(Powers) + L::ELEMS * (int)sizeof(T);
@@ -615,20 +655,26 @@ int launch(const ChunkArgs& g, hipStream_t s) {
         int dev = 0;
         if (hipError_t e = hipGetDevice(&dev)) return (int)e;
         if (dev >= 64 || !done[dev].load(std::memory_order_acquire)) {       // (an attribute of the device; a racing first call repeats it)
-            if (hipError_t e = hipFuncSetAttribute((const void*)chunk_kernel<T, DP, MODE>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes)) return (int)e;
+            if (hipError_t e = hipFuncSetAttribute((const void*)chunk_kernel<T, DP, MODE, VEC>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes)) return (int)e;
             if (dev < 64) done[dev].store(true, std::memory_order_release);
         }
     }
-    hipLaunchKernelGGL((chunk_kernel<T, DP, MODE>), dim3((unsigned)blocks), dim3(L::NT), bytes, s, g);
+    hipLaunchKernelGGL((chunk_kernel<T, DP, MODE, VEC>), dim3((unsigned)blocks), dim3(L::NT), bytes, s, g);
     GAST_CHECK_LAUNCH();
     return 0;
 }
-template <typename T, int MODE>
+template <typename T, int MODE, bool VEC>
 int launch_dp(const ChunkArgs& g, int dp, hipStream_t s) {
-    if (dp == 32) return launch<T, 32, MODE>(g, s);
-    if (dp == 64) return launch<T, 64, MODE>(g, s);
-    if constexpr (MODE != THREE) return launch<T, 128, MODE>(g, s);
+    if (dp == 32) return launch<T, 32, MODE, VEC>(g, s);
+    if (dp == 64) return launch<T, 64, MODE, VEC>(g, s);
+    if constexpr (MODE != THREE) return dp == 96 ? launch<T, 96, MODE, VEC>(g, s) : launch<T, 128, MODE, VEC>(g, s);
     return GAST_EINVAL;
+}
+// VEC: every tensor that is brought in has whole vectors
+template <typename T, int MODE>
+int launch_any(const ChunkArgs& g, int dp, hipStream_t s) {
+    const bool vec = (MODE == SUMS || g.al[0]) && g.al[1] && g.al[2] && (MODE == ONE || MODE == SUMS || g.al[3]);
+    return vec ? launch_dp<T, MODE, true>(g, dp, s) : launch_dp<T, MODE, false>(g, dp, s);
 }
 
 ChunkArgs chunk_args(const gast_decay_args& g, const Cut& c) {
@@ -637,7 +683,12 @@ ChunkArgs chunk_args(const gast_decay_args& g, const Cut& c) {
     return a;
 }
 int on16(const gast_seq& s, int dtype) { return seq_align(s, dtype == GAST_F32 ? 4 : 2, dtype == GAST_F32 ? 4 : 8) == (dtype == GAST_F32 ? 4 : 8); }
-void put_in(ChunkArgs& a, int i, const gast_seq& s, int D, int dtype) { a.in[i] = s; a.D[i] = D; a.al[i] = on16(s, dtype); }
+void put_in(ChunkArgs& a, int i, const gast_seq& s, int D, int dtype) {
+    const int es = dtype == GAST_F32 ? 4 : 2;
+    a.in[i] = s;
+    a.D[i] = D;
+    a.al[i] = on16(s, dtype) && D % (16 / es) == 0 && s.t >= 0 && (CT * s.t + GAST_DECAY_MAX_D) * es < (1L << 31);      // (whole vectors, 32-bit offsets)
+}
 Role role_of(const gast_seq& out, int D1, int D2, int reverse, float scale, int dtype) {
     Role r = {};
     r.out = out; r.D1 = D1; r.D2 = D2; r.al = out.p ? on16(out, dtype) : 0; r.reverse = reverse;
@@ -654,7 +705,7 @@ int states(const gast_decay_args& g, const Cut& c, const gast_seq& b, const gast
     a.role[0] = role_of(gast_seq{}, g.Dk, g.Dv, reverse, g.scale, g.dtype);
     a.role[0].xout = ws;
     a.skip_last = !last;
-    if (int rc = launch_dp<T, SUMS>(a, c.dp, s)) return rc;
+    if (int rc = launch_any<T, SUMS>(a, c.dp, s)) return rc;
     JoinArgs j = {ws, first, last, g.log_decay, g.lengths, g.T, g.J, g.H, c.nseg, c.L, g.Dk * g.Dv, reverse};
     hipLaunchKernelGGL(join_kernel, dim3((unsigned)((long)g.B * g.J * g.H), (unsigned)((j.size + 255) / 256)), dim3(256), 0, s, j);
     GAST_CHECK_LAUNCH();
@@ -676,7 +727,7 @@ int forward(const gast_decay_args& g, hipStream_t s) {
         a.role[0].xin = g.state;
         a.role[0].xout = g.state_out;
     }
-    return launch_dp<T, ONE>(a, c.dp, s);
+    return launch_any<T, ONE>(a, c.dp, s);
 }
 
 template <typename T>
@@ -706,15 +757,15 @@ int backward(const gast_decay_args& g, hipStream_t s) {
     dq.turn = 1;
     if (g.T <= CT && c.dp <= 64) {
         a.role[2] = dq;
-        return launch_dp<T, THREE>(a, c.dp, s);
+        return launch_any<T, THREE>(a, c.dp, s);
     }
-    if (int rc = launch_dp<T, TWO>(a, c.dp, s)) return rc;
+    if (int rc = launch_any<T, TWO>(a, c.dp, s)) return rc;
     ChunkArgs d = chunk_args(g, c);
     put_in(d, 0, g.d_o, g.Dv, g.dtype);
     put_in(d, 1, g.v, g.Dv, g.dtype);
     put_in(d, 2, g.k, g.Dk, g.dtype);
     d.role[0] = dq;
-    return launch_dp<T, ONE>(d, c.dp, s);
+    return launch_any<T, ONE>(d, c.dp, s);
 }
 
 }  // namespace
