@@ -65,15 +65,27 @@ __device__ __forceinline__ void unpack(const Frag<bf16_t>& f, float (&v)[16]) {
         h16x2_unpack(f.x[q].z, v[8 * q + 4], v[8 * q + 5]); h16x2_unpack(f.x[q].w, v[8 * q + 6], v[8 * q + 7]);
     }
 }
+// two bf16 of two values, and what they leave of them (exact).  The empty statement keeps hipcc from converting the low half a second time.
+__device__ __forceinline__ uint32_t take2(float& a, float& b) {
+    uint32_t u = pack_bf16x2(a, b);
+    asm("" : "+v"(u));
+    a -= __uint_as_float(u << 16);
+    b -= __uint_as_float(u & 0xffff0000u);
+    return u;
+}
 template <typename V> __device__ __forceinline__ Split split16(const V& v) {
     Split s;
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
-        uint2 h0, l0, h1, l1;
-        split_pair4<1>(v[8 * q], v[8 * q + 1], v[8 * q + 2], v[8 * q + 3], h0, l0);
-        split_pair4<1>(v[8 * q + 4], v[8 * q + 5], v[8 * q + 6], v[8 * q + 7], h1, l1);
-        s.hi[q] = make_uint4(h0.x, h0.y, h1.x, h1.y);
-        s.lo[q] = make_uint4(l0.x, l0.y, l1.x, l1.y);
+        uint32_t h[4], l[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float a = v[8 * q + 2 * e], b = v[8 * q + 2 * e + 1];
+            h[e] = take2(a, b);
+            l[e] = pack_bf16x2(a, b);
+        }
+        s.hi[q] = make_uint4(h[0], h[1], h[2], h[3]);
+        s.lo[q] = make_uint4(l[0], l[1], l[2], l[3]);
     }
     return s;
 }
@@ -148,10 +160,7 @@ template <typename V> __device__ __forceinline__ Parts parts16(const V& v) {
             uint32_t u[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                float &a = w[8 * q + 2 * e], &b = w[8 * q + 2 * e + 1];
-                u[e] = pack_bf16x2(a, b);
-                a -= __uint_as_float(u[e] << 16);           // (exact)
-                b -= __uint_as_float(u[e] & 0xffff0000u);
+                u[e] = take2(w[8 * q + 2 * e], w[8 * q + 2 * e + 1]);
             }
             s.x[k][q] = make_uint4(u[0], u[1], u[2], u[3]);
         }
@@ -347,15 +356,14 @@ template <int DP, int MODE> struct Lay {
 
 // exp(g n) to two steps of fp32, however long n is: the product's rounding is carried along
 __device__ __forceinline__ float power(float g, float n) {
-    if (n == 0.f) return 1.f;                              // (minus infinity: lambda^0 is 1 all the same)
-    const float x = g * n, rest = fmaf(g, n, -x), e = expf(x);
-    return e > 0.f && e < INFINITY ? fmaf(e, rest, e) : e;
+    const float x = g * n, rest = fmaf(g, n, -x), e = expf(x), p = fmaf(e, rest, e);
+    return n == 0.f ? 1.f : e > 0.f && e < INFINITY ? p : e;        // (minus infinity: lambda^0 is 1 all the same)
 }
-struct Powers { float up[CT + 4], down[CT + 4]; };        // lambda^k, k = 0 .. 32; down[k] = lambda^(31 - k)
+struct Powers { float up[CT + 4], down[2 * CT]; };        // up[k] = lambda^k, k = 0 .. 32; down[k] = lambda^(31 - k), 0 behind
 
 // The state is held as X = acc * Xh with acc = lambda^(tokens since it was last brought up to date): decaying the accumulators costs nothing
 // until acc leaves [2^-8, 2^8].  What enters is divided by acc, what leaves multiplied.
-template <typename T, int DP, int MODE, bool VEC>
+template <typename T, int DP, int MODE, bool VEC, bool STATE>
 __global__ void __launch_bounds__((Lay<DP, MODE>::NT), 2) chunk_kernel(const ChunkArgs g) {
     using L = Lay<DP, MODE>;
     constexpr int NW = L::NW, RS = L::RS, G = DP / 32;
@@ -418,14 +426,17 @@ __global__ void __launch_bounds__((Lay<DP, MODE>::NT), 2) chunk_kernel(const Chu
     if (tid <= CT) {
         const float p = power(lg, (float)tid);
         pw.up[tid] = p;
-        if (tid < CT) pw.down[CT - 1 - tid] = p;
+        if (tid < CT) {
+            pw.down[CT - 1 - tid] = p;
+            pw.down[CT + tid] = 0.f;
+        }
     }
     f32x16 X[G];
     float acc = 1.f;
     int since = 0;
 #pragma unroll
     for (int q = 0; q < G; ++q) X[q] = f32x16{};
-    if (MODE != SUMS && ro.xin && works) {
+    if (STATE && MODE != SUMS && ro.xin && works) {
         const float* xin = ro.xin + ((long)hd * g.nseg + seg) * (D1 * D2);
         const int sd = ro.turn ? 1 : D2;
         xin += min(c0, D2 - 1) * (ro.turn ? D1 : 1);       // (columns behind the last repeat it: nothing of theirs is stored)
@@ -438,90 +449,79 @@ __global__ void __launch_bounds__((Lay<DP, MODE>::NT), 2) chunk_kernel(const Chu
                 X[q][r] = d < D1 ? x : 0.f;
             }
     }
-    const bool carries = MODE == SUMS || (MODE == ONE ? ro.xin || nchunk > 1 : true);      // is there a state to meet a?
-    const bool wanted = MODE == SUMS || (ro.xout && (MODE != THREE || grp < 2));             // ... and is the last one wanted?
     if (nchunk) place(c_first);
     __syncthreads();
-    // powers that every chunk uses: lambda^|i - j| of the scores this lane holds, for tokens j = 8 (r / 4) + 4 half + r % 4 and i = col
+    // lambda^|i - j| of the scores this lane holds, for tokens j = 8 (r / 4) + 4 half + r % 4 and i = col; 0 where i does not see j
     float pd[16];
-    const uint32_t seen = (rev ? ~0u << col : ~0u >> (31 - col)) >> (4 * half);      // bit 8 (r / 4) + r % 4: token j of register r counts for i
     if constexpr (MODE != SUMS)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            const int k = 8 * (r >> 2) + 4 * half + (r & 3), gap = rev ? k - col : col - k;
-            pd[r] = pw.up[abs(gap)] * ro.fp;               // (the others are masked)
+            const int gap = (8 * (r >> 2) + 4 * half + (r & 3) - col) * (rev ? 1 : -1);
+            pd[r] = gap >= 0 ? pw.up[abs(gap)] * ro.fp : 0.f;
         }
     T* const O = (T*)ro.out.p + (MODE == SUMS ? 0 : seq_at(ro.out, b, 0, j, h));
     for (int c = 0; c < nchunk; ++c) {
-        const int ch = rev ? nchunk - 1 - c : c, t0 = s0 + ch * CT, n = min(CT, e1 - t0);
-        if (c + 1 < nchunk) fetch(rev ? ch - 1 : ch + 1);
+        const int ch = rev ? nchunk - 1 - c : c, next = c + 1 < nchunk ? (rev ? ch - 1 : ch + 1) : ch, t0 = s0 + ch * CT, n = min(CT, e1 - t0);
+        // backward in time the gradient of the last state meets the last token undecayed
+        const int first = rev && t0 + n == len ? 1 : 0;
+        const float before = acc;
+        float decay = 1.f;
+        bool renew = false;
+        if constexpr (STATE) {
+            since += n - first;
+            decay = power(lg, (float)since);
+            renew = !(decay > 0x1p-8f && decay < 0x1p8f);
+            acc = renew ? 1.f : decay;
+            since = renew ? 0 : since;
+        }
+        if constexpr (STATE) fetch(next);                  // (the last chunk once more: no branch here)
         if (works) {
-            // backward in time the gradient of the last state meets the last token undecayed
-            const int first = rev && t0 + n == len ? 1 : 0;
-            f32x16 Y = {};
-            float p[16];
-            if constexpr (MODE != SUMS) {
-                f32x16 P = {};
+            // ---- P[j][i] = b_j a_i, Y[e][i] = sum_d X[d][e] a_i[d]; meanwhile c as it enters the state
+            f32x16 P = {}, Y = {};
+            if constexpr (MODE != SUMS)
 #pragma unroll
                 for (int q = 0; q < G; ++q) {
                     const Frag<T> fa = ld_frag(ta + col * RS + 32 * q, half), fb = ld_frag(tb + col * RS + 32 * q, half);
-                    mma(P, fb, fa);                            // P[j][i] = b_j a_i
-                    if (carries) mma_fs(Y, X[q], fa);          // Y[e][i] = sum_d X[d][e] a_i[d]
+                    mma(P, fb, fa);
+                    if constexpr (STATE) mma_fs(Y, X[q], fa);
                 }
-                const float od = pw.up[max((rev ? n - 1 - col : col) + 1 - first, 0)] * ro.fo * acc;
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    p[r] = seen >> (8 * (r >> 2) + (r & 3)) & 1 ? P[r] * pd[r] : 0.f;
-                    Y[r] *= od;
-                }
-            }
             const Frag<T> fc = ld_frag(tc + col * TS, half);
-            if constexpr (MODE != SUMS) {
-                Prepared<T> pp;
-                pp.set(p);
-                mma_sf(Y, fc, pp.v);                           // Y[e][i] += sum_j c_j[e] P[j][i]
-            }
-            if (wanted || c + 1 < nchunk) {
-                const int m = n - first;
-                since += m;
-                acc = power(lg, (float)since);
-                if (!(acc > 0x1p-8f && acc < 0x1p8f)) {
-#pragma unroll
-                    for (int q = 0; q < G; ++q)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) X[q][r] *= acc;
-                    acc = 1.f;
-                    since = 0;
-                }
+            Exact<T> pv;
+            if constexpr (STATE) {
                 float v[16];
                 unpack(fc, v);
                 const float in_acc = ro.fk / acc;
-                const float* kd = rev ? pw.up : pw.down;           // token k enters with lambda^k, or lambda^(n - 1 - k)
-                if (rev || n == CT) {
+                const float* kd = (rev ? pw.up : pw.down + CT - n) + 4 * half;         // token k enters with lambda^k, or lambda^(n - 1 - k)
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const float4 f = *(const float4*)(kd + 8 * q + 4 * half);
-                        v[4 * q] *= f.x * in_acc; v[4 * q + 1] *= f.y * in_acc; v[4 * q + 2] *= f.z * in_acc; v[4 * q + 3] *= f.w * in_acc;
-                    }
-                } else {
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) v[r] *= pw.up[max(n - 1 - (8 * (r >> 2) + 4 * half + (r & 3)), 0)] * in_acc;
-                }
-                Exact<T> pv;
+                for (int r = 0; r < 16; ++r) v[r] *= kd[8 * (r >> 2) + (r & 3)] * in_acc;
                 pv.set(v);
+                if (renew)
+#pragma unroll
+                    for (int q = 0; q < G; ++q) X[q] *= decay;
+            }
+            // ---- X += b c; meanwhile the scores, and Y[e][i] += sum_j c_j[e] P[j][i]
+            if constexpr (STATE)
 #pragma unroll
                 for (int q = 0; q < G; ++q) mma_sf(X[q], ld_frag(tbT + (32 * q + col) * TS, half), pv.v);
+            if constexpr (MODE != SUMS) {
+                float p[16];
+#pragma unroll
+                for (int r = 0; r < 16; ++r) p[r] = pd[r] != 0.f ? P[r] * pd[r] : 0.f;
+                Prepared<T> pp;
+                pp.set(p);
+                if constexpr (STATE) Y *= pw.up[max((rev ? n - 1 - col : col) + 1 - first, 0)] * ro.fo * before;
+                mma_sf(Y, fc, pp.v);
+                put_tile<T>(Y, to, O, ro.out.t, t0, n, wv * 32, D2, ro.al, lane);
             }
-            if constexpr (MODE != SUMS) put_tile<T>(Y, to, O, ro.out.t, t0, n, wv * 32, D2, ro.al, lane);
         }
         if (c + 1 < nchunk) {
             __syncthreads();
-            place(rev ? ch - 1 : ch + 1);
+            place(next);
             __syncthreads();
         }
     }
     if (MODE != SUMS && s1 > max(e1, s0)) put_zeros<T>(O, ro.out.t, max(e1, s0), s1, D2, ro.al, tid - grp * NW * 64, NW * 64);
-    if (wanted && works) {
+    if (STATE && ro.xout && works) {
         float* xo = ro.xout + ((long)hd * g.nseg + seg) * (D1 * D2);
         const float f = MODE != SUMS && rev && len ? pw.up[1] * acc : acc;
         if (c0 >= D2) return;
@@ -643,7 +643,7 @@ Cut cut(long heads, int T, int Dk, int Dv) {
     return c;
 }
 
-template <typename T, int DP, int MODE, bool VEC>
+template <typename T, int DP, int MODE, bool VEC, bool STATE>
 int launch(const ChunkArgs& g, hipStream_t s) {
     using L = Lay<DP, MODE>;
     constexpr int bytes = (int)sizeof(Powers) + L::ELEMS * (int)sizeof(T);
@@ -655,26 +655,31 @@ int launch(const ChunkArgs& g, hipStream_t s) {
         int dev = 0;
         if (hipError_t e = hipGetDevice(&dev)) return (int)e;
         if (dev >= 64 || !done[dev].load(std::memory_order_acquire)) {       // (an attribute of the device; a racing first call repeats it)
-            if (hipError_t e = hipFuncSetAttribute((const void*)chunk_kernel<T, DP, MODE, VEC>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes)) return (int)e;
+            if (hipError_t e = hipFuncSetAttribute((const void*)chunk_kernel<T, DP, MODE, VEC, STATE>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes)) return (int)e;
             if (dev < 64) done[dev].store(true, std::memory_order_release);
         }
     }
-    hipLaunchKernelGGL((chunk_kernel<T, DP, MODE, VEC>), dim3((unsigned)blocks), dim3(L::NT), bytes, s, g);
+    hipLaunchKernelGGL((chunk_kernel<T, DP, MODE, VEC, STATE>), dim3((unsigned)blocks), dim3(L::NT), bytes, s, g);
     GAST_CHECK_LAUNCH();
     return 0;
 }
-template <typename T, int MODE, bool VEC>
+template <typename T, int MODE, bool VEC, bool STATE>
 int launch_dp(const ChunkArgs& g, int dp, hipStream_t s) {
-    if (dp == 32) return launch<T, 32, MODE, VEC>(g, s);
-    if (dp == 64) return launch<T, 64, MODE, VEC>(g, s);
-    if constexpr (MODE != THREE) return dp == 96 ? launch<T, 96, MODE, VEC>(g, s) : launch<T, 128, MODE, VEC>(g, s);
+    if (dp == 32) return launch<T, 32, MODE, VEC, STATE>(g, s);
+    if (dp == 64) return launch<T, 64, MODE, VEC, STATE>(g, s);
+    if constexpr (MODE != THREE) return dp == 96 ? launch<T, 96, MODE, VEC, STATE>(g, s) : launch<T, 128, MODE, VEC, STATE>(g, s);
     return GAST_EINVAL;
 }
-// VEC: every tensor that is brought in has whole vectors
+// VEC: every tensor that is brought in has whole vectors.  STATE: there is a state to start from, to return or to hand to a second chunk.
 template <typename T, int MODE>
 int launch_any(const ChunkArgs& g, int dp, hipStream_t s) {
     const bool vec = (MODE == SUMS || g.al[0]) && g.al[1] && g.al[2] && (MODE == ONE || MODE == SUMS || g.al[3]);
-    return vec ? launch_dp<T, MODE, true>(g, dp, s) : launch_dp<T, MODE, false>(g, dp, s);
+    if constexpr (MODE == ONE || MODE == THREE) {
+        bool state = g.T > CT;
+        for (const Role& r : g.role) state = state || r.xin || r.xout;
+        if (!state) return vec ? launch_dp<T, MODE, true, false>(g, dp, s) : launch_dp<T, MODE, false, false>(g, dp, s);
+    }
+    return vec ? launch_dp<T, MODE, true, true>(g, dp, s) : launch_dp<T, MODE, false, true>(g, dp, s);
 }
 
 ChunkArgs chunk_args(const gast_decay_args& g, const Cut& c) {
