@@ -184,6 +184,26 @@ __device__ __forceinline__ void mma_sf(f32x16& c, const Frag<bf16_t>& a, const P
         for (int k = 2; k >= 0; --k) c = mfma_pair<1>(a.x[q], b.x[k][q], c);
 #endif
 }
+// X[q] += A[q] B for every q, one after the other: none waits for the one before
+template <int G> __device__ __forceinline__ void mma_into(f32x16 (&X)[G], const Frag<float> (&a)[G], const float (&b)[16]) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+#pragma unroll
+        for (int q = 0; q < G; ++q) X[q] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[q].x[i], b[i], X[q], 0, 0, 0);
+}
+template <int G> __device__ __forceinline__ void mma_into(f32x16 (&X)[G], const Frag<bf16_t> (&a)[G], const Parts& b) {
+#ifdef GAST_H16_F16
+#pragma unroll
+    for (int q = 0; q < G; ++q) mma_sf(X[q], a[q], b);
+#else
+#pragma unroll
+    for (int k = 2; k >= 0; --k)
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int q = 0; q < G; ++q) X[q] = mfma_pair<1>(a[q].x[s], b.x[k][s], X[q]);
+#endif
+}
 // the fp32 side of mma_sf, prepared once where several products share it: scores in two parts, what enters a state in three
 template <typename T> struct Prepared;
 template <> struct Prepared<float> {
@@ -350,8 +370,7 @@ template <int DP, int MODE> struct Lay {
     static constexpr int NW = DP / 32, RS = DP + 4, ROWS = CT * RS, TURN = DP * TS;
     static constexpr int GROUPS = MODE == TWO ? 2 : MODE == THREE ? 3 : 1, NT = GROUPS * NW * 64;
     static constexpr int NROWS = MODE == ONE ? 2 : MODE == SUMS ? 0 : 4, NTURN = MODE == THREE ? 3 : 2;
-    static constexpr int OUT = MODE == TWO || MODE == THREE ? GROUPS * NW * 32 * TS : 0;
-    static constexpr int ELEMS = NROWS * ROWS + NTURN * TURN + OUT;
+    static constexpr int OUT = MODE == TWO || MODE == THREE ? GROUPS * NW * 32 * TS : 0, TILES = NROWS * ROWS + NTURN * TURN;
 };
 
 // exp(g n) to two steps of fp32, however long n is: the product's rounding is carried along
@@ -359,19 +378,32 @@ __device__ __forceinline__ float power(float g, float n) {
     const float x = g * n, rest = fmaf(g, n, -x), e = expf(x), p = fmaf(e, rest, e);
     return n == 0.f ? 1.f : e > 0.f && e < INFINITY ? p : e;        // (minus infinity: lambda^0 is 1 all the same)
 }
-struct Powers { float up[CT + 4], down[2 * CT]; };        // up[k] = lambda^k, k = 0 .. 32; down[k] = lambda^(31 - k), 0 behind
+// The state is held as X = unit[p] * Xh, unit[p] = lambda^(32 p), p = chunks since the accumulators were last brought up to date: decaying them
+// costs nothing until unit leaves [2^-8, 2^8].  What enters is divided by the unit, what leaves multiplied.
+constexpr int PERIOD = 32;                                 // ... or until this many chunks
+struct Powers {
+    float up[CT + 4];                                      // lambda^k, k = 0 .. 32
+    float down[2 * CT];                                    // lambda^(31 - k), 0 behind
+    float unit[PERIOD + 4], per_unit[PERIOD + 4];
+};
+template <typename T, int DP, int MODE, bool STATE> struct Lds {
+    using L = Lay<DP, MODE>;
+    // two sets of tiles (one barrier a chunk instead of two) where the waves that the registers allow still fit: 20 KB a wave
+    static constexpr int NBUF = STATE && 2 * L::TILES * (int)sizeof(T) + L::OUT * (int)sizeof(T) <= 20 * 1024 * L::GROUPS * L::NW ? 2 : 1;
+    Powers pw;
+    T tiles[NBUF * L::TILES + L::OUT];
+};
 
-// The state is held as X = acc * Xh with acc = lambda^(tokens since it was last brought up to date): decaying the accumulators costs nothing
-// until acc leaves [2^-8, 2^8].  What enters is divided by acc, what leaves multiplied.
+
 template <typename T, int DP, int MODE, bool VEC, bool STATE>
 __global__ void __launch_bounds__((Lay<DP, MODE>::NT), 2) chunk_kernel(const ChunkArgs g) {
     using L = Lay<DP, MODE>;
     constexpr int NW = L::NW, RS = L::RS, G = DP / 32;
     constexpr bool BWD = MODE == TWO || MODE == THREE;
     extern __shared__ __align__(16) char lds[];
-    Powers& pw = *(Powers*)lds;
-    T* const rows0 = (T*)(lds + sizeof(Powers));
-    T* const turn0 = rows0 + L::NROWS * L::ROWS;
+    using M = Lds<T, DP, MODE, STATE>;
+    M& m = *(M*)lds;
+    constexpr int NBUF = M::NBUF, TURN0 = L::NROWS * L::ROWS;
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), grp = wave / NW, wv = wave % NW;
     const uint32_t heads = (uint32_t)g.B * g.J * g.H, bid = xcd_remap(blockIdx.x, gridDim.x);
@@ -385,10 +417,8 @@ __global__ void __launch_bounds__((Lay<DP, MODE>::NT), 2) chunk_kernel(const Chu
     const float lg = g.log_decay[h];
     // ---- roles: dv (a, b, c) = (k, q, do), dk (v, do, q), dq (do, v, k); turned tiles of BWD: q, do (, k)
     const int ia = BWD ? (grp == 0 ? 2 : grp == 1 ? 3 : 1) : 0, ib = BWD ? (grp == 0 ? 0 : grp == 1 ? 1 : 3) : 1, ic = BWD ? (grp == 0 ? 1 : grp == 1 ? 0 : 2) : 2;
-    const T *ta = rows0 + ia * L::ROWS, *tb = rows0 + ib * L::ROWS;
-    const T *tbT = turn0 + (BWD ? ib : 0) * L::TURN;
-    T* const tc = turn0 + (BWD ? ic : 1) * L::TURN + wv * 32 * TS;                 // this wave's 32 columns of c
-    T* const to = BWD ? turn0 + L::NTURN * L::TURN + wave * 32 * TS : tc;
+    const int oa = ia * L::ROWS, ob = ib * L::ROWS, obT = TURN0 + (BWD ? ib : 0) * L::TURN;       // offsets in a set of tiles
+    const int oc = TURN0 + (BWD ? ic : 1) * L::TURN + wv * 32 * TS;                               // (this wave's 32 columns of c)
     const int c0 = wv * 32 + col, D1 = ro.D1, D2 = ro.D2;
     const bool works = wv * 32 < D2;
 
@@ -410,30 +440,34 @@ __global__ void __launch_bounds__((Lay<DP, MODE>::NT), 2) chunk_kernel(const Chu
 #pragma unroll
             for (int i = 0; i < NS; ++i) bring<T>(stage[i], in[i], t0, n, wv, lane);      // (THREE: two groups bring in nothing new the second time)
     };
-    auto place = [&](int c) {
+    auto place = [&](int c, T* tiles) {
         const int t0 = s0 + c * CT, n = min(CT, e1 - t0);
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
             if (st[i] < 0) continue;
             if constexpr (VEC) { if (!whole || n < CT) trim<T>(stage[i], in[i], n, wv, lane); }
             else bring_odd<T>(stage[i], in[i], t0, n, wv, lane);
-            if (MODE == ONE ? i < 2 : MODE != SUMS) stage[i].template rows<RS>(rows0 + st[i] * L::ROWS, wv, lane);
-            if (MODE == ONE ? i > 0 : MODE == SUMS || st[i] < L::NTURN) stage[i].turned(turn0 + (BWD ? st[i] : st[i] - 1) * L::TURN, wv, lane);
+            if (MODE == ONE ? i < 2 : MODE != SUMS) stage[i].template rows<RS>(tiles + st[i] * L::ROWS, wv, lane);
+            if (MODE == ONE ? i > 0 : MODE == SUMS || st[i] < L::NTURN) stage[i].turned(tiles + TURN0 + (BWD ? st[i] : st[i] - 1) * L::TURN, wv, lane);
         }
     };
     const int c_first = rev && MODE != THREE ? nchunk - 1 : 0;
     if (nchunk) fetch(c_first);
+    Powers& pw = m.pw;
     if (tid <= CT) {
-        const float p = power(lg, (float)tid);
+        const float p = power(lg, (float)tid), u = power(lg, 32.f * tid);
         pw.up[tid] = p;
+        pw.unit[tid] = u;
+        pw.per_unit[tid] = 1.f / u;
         if (tid < CT) {
             pw.down[CT - 1 - tid] = p;
             pw.down[CT + tid] = 0.f;
         }
     }
+    const float steps = 5.545f / (32.f * fabsf(lg));       // ln 2^8
+    const int period = steps >= PERIOD ? PERIOD : max((int)steps, 1);
+    int p = 0;
     f32x16 X[G];
-    float acc = 1.f;
-    int since = 0;
 #pragma unroll
     for (int q = 0; q < G; ++q) X[q] = f32x16{};
     if (STATE && MODE != SUMS && ro.xin && works) {
@@ -449,7 +483,7 @@ __global__ void __launch_bounds__((Lay<DP, MODE>::NT), 2) chunk_kernel(const Chu
                 X[q][r] = d < D1 ? x : 0.f;
             }
     }
-    if (nchunk) place(c_first);
+    if (nchunk) place(c_first, m.tiles);
     __syncthreads();
     // lambda^|i - j| of the scores this lane holds, for tokens j = 8 (r / 4) + 4 half + r % 4 and i = col; 0 where i does not see j
     float pd[16];
@@ -462,26 +496,21 @@ __global__ void __launch_bounds__((Lay<DP, MODE>::NT), 2) chunk_kernel(const Chu
     T* const O = (T*)ro.out.p + (MODE == SUMS ? 0 : seq_at(ro.out, b, 0, j, h));
     for (int c = 0; c < nchunk; ++c) {
         const int ch = rev ? nchunk - 1 - c : c, next = c + 1 < nchunk ? (rev ? ch - 1 : ch + 1) : ch, t0 = s0 + ch * CT, n = min(CT, e1 - t0);
+        T* const tiles = m.tiles + (NBUF == 2 ? (c & 1) * L::TILES : 0);
         // backward in time the gradient of the last state meets the last token undecayed
-        const int first = rev && t0 + n == len ? 1 : 0;
-        const float before = acc;
-        float decay = 1.f;
-        bool renew = false;
-        if constexpr (STATE) {
-            since += n - first;
-            decay = power(lg, (float)since);
-            renew = !(decay > 0x1p-8f && decay < 0x1p8f);
-            acc = renew ? 1.f : decay;
-            since = renew ? 0 : since;
-        }
+        const int first = rev && t0 + n == len ? 1 : 0, steps_on = n - first;
+        const bool renew = p + 1 >= period || steps_on < CT;
+        const int pa = renew ? 0 : p + 1;                   // the unit afterwards
         if constexpr (STATE) fetch(next);                  // (the last chunk once more: no branch here)
         if (works) {
+            const T *ta = tiles + oa + col * RS, *tb = tiles + ob + col * RS, *tbT = tiles + obT + col * TS;
+            T* const tc = tiles + oc;
             // ---- P[j][i] = b_j a_i, Y[e][i] = sum_d X[d][e] a_i[d]; meanwhile c as it enters the state
             f32x16 P = {}, Y = {};
             if constexpr (MODE != SUMS)
 #pragma unroll
                 for (int q = 0; q < G; ++q) {
-                    const Frag<T> fa = ld_frag(ta + col * RS + 32 * q, half), fb = ld_frag(tb + col * RS + 32 * q, half);
+                    const Frag<T> fa = ld_frag(ta + 32 * q, half), fb = ld_frag(tb + 32 * q, half);
                     mma(P, fb, fa);
                     if constexpr (STATE) mma_fs(Y, X[q], fa);
                 }
@@ -490,40 +519,48 @@ __global__ void __launch_bounds__((Lay<DP, MODE>::NT), 2) chunk_kernel(const Chu
             if constexpr (STATE) {
                 float v[16];
                 unpack(fc, v);
-                const float in_acc = ro.fk / acc;
-                const float* kd = (rev ? pw.up : pw.down + CT - n) + 4 * half;         // token k enters with lambda^k, or lambda^(n - 1 - k)
+                const float w = ro.fk * pw.per_unit[pa];
+                const float* in_by = (rev ? pw.up : pw.down + CT - n) + 4 * half;      // token k enters with lambda^k, or lambda^(n - 1 - k)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) v[r] *= kd[8 * (r >> 2) + (r & 3)] * in_acc;
+                for (int r = 0; r < 16; ++r) v[r] *= in_by[8 * (r >> 2) + (r & 3)] * w;
                 pv.set(v);
-                if (renew)
+                if (renew) {
+                    const float f = pw.unit[p] * pw.up[steps_on];
 #pragma unroll
-                    for (int q = 0; q < G; ++q) X[q] *= decay;
+                    for (int q = 0; q < G; ++q) X[q] *= f;
+                }
             }
             // ---- X += b c; meanwhile the scores, and Y[e][i] += sum_j c_j[e] P[j][i]
-            if constexpr (STATE)
+            if constexpr (STATE) {
+                Frag<T> fk[G];
 #pragma unroll
-                for (int q = 0; q < G; ++q) mma_sf(X[q], ld_frag(tbT + (32 * q + col) * TS, half), pv.v);
+                for (int q = 0; q < G; ++q) fk[q] = ld_frag(tbT + 32 * q * TS, half);
+                mma_into<G>(X, fk, pv.v);
+            }
             if constexpr (MODE != SUMS) {
-                float p[16];
+                float sc[16];
 #pragma unroll
-                for (int r = 0; r < 16; ++r) p[r] = pd[r] != 0.f ? P[r] * pd[r] : 0.f;
+                for (int r = 0; r < 16; ++r) sc[r] = pd[r] != 0.f ? P[r] * pd[r] : 0.f;
                 Prepared<T> pp;
-                pp.set(p);
-                if constexpr (STATE) Y *= pw.up[max((rev ? n - 1 - col : col) + 1 - first, 0)] * ro.fo * before;
+                pp.set(sc);
+                if constexpr (STATE) Y *= pw.up[max((rev ? n - 1 - col : col) + 1 - first, 0)] * pw.unit[p] * ro.fo;
                 mma_sf(Y, fc, pp.v);
-                put_tile<T>(Y, to, O, ro.out.t, t0, n, wv * 32, D2, ro.al, lane);
+                put_tile<T>(Y, BWD ? m.tiles + NBUF * L::TILES + wave * 32 * TS : tc, O, ro.out.t, t0, n, wv * 32, D2, ro.al, lane);
             }
         }
-        if (c + 1 < nchunk) {
-            __syncthreads();
-            place(next);
-            __syncthreads();
+        if constexpr (STATE) {
+            p = pa;
+            if (c + 1 < nchunk) {
+                if constexpr (NBUF == 1) __syncthreads();
+                place(next, m.tiles + (NBUF == 2 ? ((c + 1) & 1) * L::TILES : 0));
+                __syncthreads();
+            }
         }
     }
     if (MODE != SUMS && s1 > max(e1, s0)) put_zeros<T>(O, ro.out.t, max(e1, s0), s1, D2, ro.al, tid - grp * NW * 64, NW * 64);
     if (STATE && ro.xout && works) {
         float* xo = ro.xout + ((long)hd * g.nseg + seg) * (D1 * D2);
-        const float f = MODE != SUMS && rev && len ? pw.up[1] * acc : acc;
+        const float f = pw.unit[p] * (MODE != SUMS && rev && len ? pw.up[1] : 1.f);
         if (c0 >= D2) return;
 #pragma unroll
         for (int q = 0; q < G; ++q)
@@ -646,7 +683,7 @@ Cut cut(long heads, int T, int Dk, int Dv) {
 template <typename T, int DP, int MODE, bool VEC, bool STATE>
 int launch(const ChunkArgs& g, hipStream_t s) {
     using L = Lay<DP, MODE>;
-    constexpr int bytes = (int)sizeof(Powers) + L::ELEMS * (int)sizeof(T);
+    constexpr int bytes = (int)sizeof(Lds<T, DP, MODE, STATE>);
     const long blocks = (long)g.B * g.J * g.H * g.nseg;
     if (blocks > 0x7fffffffL) return GAST_ERANGE;
     static_assert(bytes <= 160 * 1024, "LDS of a CU");
