@@ -16,17 +16,44 @@ namespace {
 
 constexpr int MAXV = 16;             // values of a row that one lane holds
 
-// the dropout multiplier of element e of its tensor: drop_mul for e < 2^33, beyond that the high word of e / 2 enters the key
-__device__ __forceinline__ float drop_mul64(uint32_t key, uint32_t thresh, float inv_keep, long e) {
-    const uint32_t hi = (uint32_t)((unsigned long)e >> 33);
-    const uint32_t h = hash32((uint32_t)((unsigned long)e >> 1) ^ (key + hi * 0xC2B2AE35u));
-    const uint32_t bits = (e & 1) ? (h >> 16) : (h & 0xffffu);
-    return bits >= thresh ? inv_keep : 0.f;
-}
+// the dropout multipliers of elements e .. e + VE - 1 of their tensor: drop_mul for e < 2^33, beyond that the high word of e / 2 enters the
+// key.  Two neighbours share a hash, so a vector of VE >= 2 (e even) makes VE / 2 of them.
+__device__ __forceinline__ uint32_t drop_word(uint32_t key, unsigned long pair) { return hash32((uint32_t)pair ^ (key + (uint32_t)(pair >> 32) * 0xC2B2AE35u)); }
 template <int VE>
 __device__ __forceinline__ void drop_vec(float (&m)[VE], uint32_t key, uint32_t thresh, float inv_keep, long e) {
+    if constexpr (VE == 1) {
+        const uint32_t h = drop_word(key, (unsigned long)e >> 1);
+        m[0] = ((e & 1) ? h >> 16 : h & 0xffffu) >= thresh ? inv_keep : 0.f;
+    } else {
 #pragma unroll
-    for (int i = 0; i < VE; ++i) m[i] = drop_mul64(key, thresh, inv_keep, e + i);
+        for (int i = 0; i < VE; i += 2) {
+            const uint32_t h = drop_word(key, ((unsigned long)e + i) >> 1);
+            m[i] = (h & 0xffffu) >= thresh ? inv_keep : 0.f;
+            m[i + 1] = (h >> 16) >= thresh ? inv_keep : 0.f;
+        }
+    }
+}
+// the stream's value as it is stored: x m + r rounded to fp32, and that to the type.  (The empty statement keeps the binary16 build from
+// fusing both into one instruction that rounds once, which is another value now and then.)
+template <typename T> __device__ __forceinline__ float stored(float v) {
+    asm("" : "+v"(v));
+    return Elem<T>::rnd(v);
+}
+// VE parameters from column c on (fp32, on the same alignment as the rows), or `none`
+template <int VE> __device__ __forceinline__ void ld_par(float (&w)[VE], const float* p, int c, float none) {
+    constexpr int VF = VE < 4 ? VE : 4;
+#pragma unroll
+    for (int k = 0; k < VE; k += VF) {
+        float4 u = make_float4(none, none, none, none);
+        if (p) {
+            if constexpr (VF == 4) u = *(const float4*)(p + c + k);
+            else if constexpr (VF == 2) { const float2 v = *(const float2*)(p + c + k); u.x = v.x; u.y = v.y; }
+            else u.x = p[c + k];
+        }
+        w[k] = u.x;
+        if constexpr (VF > 1) w[k + 1] = u.y;
+        if constexpr (VF > 2) { w[k + 2] = u.z; w[k + 3] = u.w; }
+    }
 }
 
 // sum over the G lanes that hold a row (G <= 64: lanes of a wave; else the whole block of G threads); every lane gets it
@@ -58,79 +85,90 @@ struct NormArgs {
     float* ws;
 };
 
-// NC vectors of VE values per lane cover the row: G * NC * VE >= C
-template <typename T, int VE, int NC, int G>
+// NC vectors of VE values per lane cover the row: G * NC * VE >= C.  A block walks over rows with gamma and beta in registers.  Loads stand
+// in straight code (a join of two paths would wait for them): lanes and groups behind the end read the last vector of the last row.
+template <typename T, int VE, int NC, int G, bool ADD>
 __global__ void __launch_bounds__(G > 256 ? G : 256) norm_fwd_kernel(const NormArgs a) {
     constexpr int GPB = G > 256 ? 1 : 256 / G;
-    __shared__ float red[2][G > 64 ? G / 64 : 1];
+    __shared__ float red[2][2][G > 64 ? G / 64 : 1];
     const int lane = threadIdx.x % G, C = a.C, nvec = C / VE;
-    const long row = (long)blockIdx.x * GPB + threadIdx.x / G;
-    const bool on = row < a.rows;
-    float s[NC][VE];
-#pragma unroll
-    for (int i = 0; i < NC; ++i)
-#pragma unroll
-        for (int e = 0; e < VE; ++e) s[i][e] = 0.f;
-    if (on) {
-        const T* x = (const T*)a.X + row * a.ldx;
-#pragma unroll
-        for (int i = 0; i < NC; ++i)
-            if (i * G + lane < nvec) ldv<VE>(s[i], x + (i * G + lane) * VE);
-        if (a.Res) {
-            const T* r = (const T*)a.Res + row * a.ldr;
-            T* so = (T*)a.S + row * a.lds;
-            float q[NC][VE];
-#pragma unroll
-            for (int i = 0; i < NC; ++i)
-                if (i * G + lane < nvec) ldv<VE>(q[i], r + (i * G + lane) * VE);
-            const uint32_t key = a.use_drop ? drop_key(a.drop, a.salt) : 0u;
-#pragma unroll
-            for (int i = 0; i < NC; ++i) {
-                if (i * G + lane >= nvec) continue;
-                const int c0 = (i * G + lane) * VE;
-                float m[VE];
-                if (a.use_drop) drop_vec<VE>(m, key, a.drop.thresh, a.drop.inv_keep, row * C + c0);
-                // one rounding of x m + r to fp32, one to the storage type; what a 0 multiplies is gone even where it is not finite
-#pragma unroll
-                for (int e = 0; e < VE; ++e)
-                    s[i][e] = Elem<T>::rnd(a.use_drop ? (m[e] == 0.f ? q[i][e] : fmaf(s[i][e], m[e], q[i][e])) : s[i][e] + q[i][e]);
-                stv<VE>(so + c0, s[i]);
-            }
-        }
-    }
-    float t = 0.f;
-#pragma unroll
-    for (int i = 0; i < NC; ++i)
-#pragma unroll
-        for (int e = 0; e < VE; ++e) t += s[i][e];
     const float inv = 1.f / (float)C;
-    const float mean = group_sum<G>(t, red[0]) * inv;
-    t = 0.f;
-#pragma unroll
-    for (int i = 0; i < NC; ++i)
-        if (i * G + lane < nvec)
-#pragma unroll
-            for (int e = 0; e < VE; ++e) t = fmaf(s[i][e] - mean, s[i][e] - mean, t);
-    const float rstd = 1.f / sqrtf(group_sum<G>(t, red[1]) * inv + a.eps);
-    if (!on) return;
-    T* y = (T*)a.Y + row * a.ldy;
+    const uint32_t key = ADD && a.use_drop ? drop_key(a.drop, a.salt) : 0u;
+    int at[NC];
+    float w[NC][VE], b[NC][VE];
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-        if (i * G + lane >= nvec) continue;
-        const int c0 = (i * G + lane) * VE;
-        float w[VE], b[VE];
-#pragma unroll
-        for (int e = 0; e < VE; ++e) {
-            w[e] = a.gamma ? a.gamma[c0 + e] : 1.f;
-            b[e] = a.beta ? a.beta[c0 + e] : 0.f;
-        }
-#pragma unroll
-        for (int e = 0; e < VE; ++e) w[e] = fmaf((s[i][e] - mean) * rstd, w[e], b[e]);
-        stv<VE>(y + c0, w);
+        at[i] = min(i * G + lane, nvec - 1) * VE;
+        ld_par<VE>(w[i], a.gamma, at[i], 1.f);
+        ld_par<VE>(b[i], a.beta, at[i], 0.f);
     }
-    if (a.mean && lane == 0) {
-        a.mean[row] = mean;
-        a.rstd[row] = rstd;
+    int par = 0;
+    for (long r0 = (long)blockIdx.x * GPB; r0 < a.rows; r0 += (long)gridDim.x * GPB, par ^= 1) {        // (block-uniform: barriers inside)
+        const long row = r0 + threadIdx.x / G, in = min(row, a.rows - 1);
+        const bool on = row < a.rows;
+        const T* x = (const T*)a.X + in * a.ldx;
+        float s[NC][VE];
+#pragma unroll
+        for (int i = 0; i < NC; ++i) ldv<VE>(s[i], x + at[i]);
+        if constexpr (ADD) {
+            const T* r = (const T*)a.Res + in * a.ldr;
+            float q[NC][VE];
+#pragma unroll
+            for (int i = 0; i < NC; ++i) ldv<VE>(q[i], r + at[i]);
+            if (a.use_drop) {
+#pragma unroll
+                for (int i = 0; i < NC; ++i) {
+                    float m[VE];
+                    drop_vec<VE>(m, key, a.drop.thresh, a.drop.inv_keep, row * C + at[i]);
+                    // what a 0 multiplies is gone even where it is not finite
+#pragma unroll
+                    for (int e = 0; e < VE; ++e) s[i][e] = stored<T>(fmaf(m[e] == 0.f ? 0.f : s[i][e], m[e], q[i][e]));
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < NC; ++i)
+#pragma unroll
+                    for (int e = 0; e < VE; ++e) s[i][e] = stored<T>(s[i][e] + q[i][e]);
+            }
+            T* so = (T*)a.S + in * a.lds;
+#pragma unroll
+            for (int i = 0; i < NC; ++i)
+                if (on && i * G + lane < nvec) stv<VE>(so + at[i], s[i]);
+        }
+        if (nvec < NC * G)
+#pragma unroll
+            for (int i = 0; i < NC; ++i)
+#pragma unroll
+                for (int e = 0; e < VE; ++e) s[i][e] = i * G + lane < nvec ? s[i][e] : 0.f;
+        float t = 0.f;
+#pragma unroll
+        for (int i = 0; i < NC; ++i)
+#pragma unroll
+            for (int e = 0; e < VE; ++e) t += s[i][e];
+        const float mean = group_sum<G>(t, red[par][0]) * inv;
+        t = 0.f;
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            float u = 0.f;
+#pragma unroll
+            for (int e = 0; e < VE; ++e) u = fmaf(s[i][e] - mean, s[i][e] - mean, u);
+            t += i * G + lane < nvec ? u : 0.f;
+        }
+        const float rstd = 1.f / sqrtf(group_sum<G>(t, red[par][1]) * inv + a.eps);
+        if (!on) continue;
+        T* y = (T*)a.Y + row * a.ldy;
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            if (i * G + lane >= nvec) continue;
+            float d[VE];
+#pragma unroll
+            for (int e = 0; e < VE; ++e) d[e] = fmaf((s[i][e] - mean) * rstd, w[i][e], b[i][e]);
+            stv<VE>(y + at[i], d);
+        }
+        if (a.mean && lane == 0) {
+            a.mean[row] = mean;
+            a.rstd[row] = rstd;
+        }
     }
 }
 
@@ -150,12 +188,13 @@ __global__ void __launch_bounds__(1024) norm_fwd_long_kernel(const NormArgs a) {
             float v = Elem<T>::ld(x + c);
             const float q = Elem<T>::ld(r + c);
             if (a.use_drop) {
-                const float m = drop_mul64(key, a.drop.thresh, a.drop.inv_keep, row * C + c);
-                v = m == 0.f ? q : fmaf(v, m, q);
+                float m[1];
+                drop_vec<1>(m, key, a.drop.thresh, a.drop.inv_keep, row * C + c);
+                v = m[0] == 0.f ? q : fmaf(v, m[0], q);
             } else {
                 v += q;
             }
-            v = Elem<T>::rnd(v);
+            v = stored<T>(v);
             Elem<T>::st(so + c, v);
             t += v;
         }
@@ -181,7 +220,8 @@ __global__ void __launch_bounds__(1024) norm_fwd_long_kernel(const NormArgs a) {
 }
 
 // g = dY gamma, xhat -> dS, dX row by row; the sums of dY xhat and dY per column stay in w0, w1 (registers of the lane that owns it)
-template <typename T, int VE, int NC, int G>
+// (ADD: there is the stream's own gradient dSt.)
+template <typename T, int VE, int NC, int G, bool ADD>
 __global__ void __launch_bounds__(G > 256 ? G : 256) norm_bwd_kernel(const NormArgs a) {
     constexpr int GPB = G > 256 ? 1 : 256 / G;
     constexpr int NT = G > 256 ? G : 256;
@@ -190,75 +230,65 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) norm_bwd_kernel(const NormA
     const int lane = threadIdx.x % G, grp = threadIdx.x / G, C = a.C, nvec = C / VE;
     const float inv = 1.f / (float)C;
     const uint32_t key = a.use_drop ? drop_key(a.drop, a.salt) : 0u;
-    float w0[NC][VE], w1[NC][VE];
+    int at[NC];
+    float w0[NC][VE], w1[NC][VE], gm[NC][VE];
 #pragma unroll
-    for (int i = 0; i < NC; ++i)
+    for (int i = 0; i < NC; ++i) {
+        at[i] = min(i * G + lane, nvec - 1) * VE;
+        ld_par<VE>(gm[i], a.gamma, at[i], 1.f);
 #pragma unroll
         for (int e = 0; e < VE; ++e) w0[i][e] = w1[i][e] = 0.f;
+    }
+    const T *dY = (const T*)(a.dY ? a.dY : a.S), *S = (const T*)a.S;            // (without dY the norm has no gradient: zeros below)
+    const long lddy = a.dY ? a.lddy : a.lds;
     int par = 0;
     for (long r0 = (long)blockIdx.x * GPB; r0 < a.rows; r0 += (long)gridDim.x * GPB, par ^= 1) {        // (block-uniform: barriers inside)
-        const long row = r0 + grp;
+        const long row = r0 + grp, in = min(row, a.rows - 1);
         const bool on = row < a.rows;
         float g[NC][VE], h[NC][VE], st[NC][VE];
 #pragma unroll
-        for (int i = 0; i < NC; ++i)
+        for (int i = 0; i < NC; ++i) ldv<VE>(h[i], S + in * a.lds + at[i]);
 #pragma unroll
-            for (int e = 0; e < VE; ++e) g[i][e] = h[i][e] = st[i][e] = 0.f;
-        float mean = 0.f, rstd = 0.f;
-        if (on) {
-            mean = a.mean[row];
-            rstd = a.rstd[row];
-            if (a.dY) {
-                const T* dy = (const T*)a.dY + row * a.lddy;
+        for (int i = 0; i < NC; ++i) ldv<VE>(g[i], dY + in * lddy + at[i]);
+        if constexpr (ADD)
 #pragma unroll
-                for (int i = 0; i < NC; ++i)
-                    if (i * G + lane < nvec) ldv<VE>(g[i], dy + (i * G + lane) * VE);
-            }
-            const T* s = (const T*)a.S + row * a.lds;
+            for (int i = 0; i < NC; ++i) ldv<VE>(st[i], (const T*)a.dSt + in * a.ldds + at[i]);
+        const float mean = a.mean[in], rstd = a.rstd[in];
+        if (!on || nvec < NC * G || !a.dY)
 #pragma unroll
             for (int i = 0; i < NC; ++i)
-                if (i * G + lane < nvec) ldv<VE>(h[i], s + (i * G + lane) * VE);
-            if (a.dSt) {
-                const T* d = (const T*)a.dSt + row * a.ldds;
 #pragma unroll
-                for (int i = 0; i < NC; ++i)
-                    if (i * G + lane < nvec) ldv<VE>(st[i], d + (i * G + lane) * VE);
-            }
-        }
+                for (int e = 0; e < VE; ++e) g[i][e] = on && i * G + lane < nvec && a.dY ? g[i][e] : 0.f;
         float t0 = 0.f, t1 = 0.f;
 #pragma unroll
-        for (int i = 0; i < NC; ++i) {
-            if (i * G + lane >= nvec) continue;
-            const int c0 = (i * G + lane) * VE;
+        for (int i = 0; i < NC; ++i)
 #pragma unroll
             for (int e = 0; e < VE; ++e) {
                 h[i][e] = (h[i][e] - mean) * rstd;
                 w0[i][e] = fmaf(g[i][e], h[i][e], w0[i][e]);
                 w1[i][e] += g[i][e];
-                if (a.gamma) g[i][e] *= a.gamma[c0 + e];
+                g[i][e] *= gm[i][e];
                 t0 += g[i][e];
                 t1 = fmaf(g[i][e], h[i][e], t1);
             }
-        }
         t0 = group_sum<G>(t0, red[par][0]) * inv;
         t1 = group_sum<G>(t1, red[par][1]) * inv;
         if (!on) continue;
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
             if (i * G + lane >= nvec) continue;
-            const int c0 = (i * G + lane) * VE;
             float d[VE];
 #pragma unroll
-            for (int e = 0; e < VE; ++e) d[e] = fmaf(rstd, g[i][e] - t0 - h[i][e] * t1, st[i][e]);
-            if (a.dS) stv<VE>((T*)a.dS + row * a.lddsum + c0, d);
+            for (int e = 0; e < VE; ++e) d[e] = ADD ? fmaf(rstd, g[i][e] - t0 - h[i][e] * t1, st[i][e]) : rstd * (g[i][e] - t0 - h[i][e] * t1);
+            if (a.dS) stv<VE>((T*)a.dS + row * a.lddsum + at[i], d);
             if (a.dX) {
                 if (a.use_drop) {
                     float m[VE];
-                    drop_vec<VE>(m, key, a.drop.thresh, a.drop.inv_keep, row * C + c0);
+                    drop_vec<VE>(m, key, a.drop.thresh, a.drop.inv_keep, row * C + at[i]);
 #pragma unroll
                     for (int e = 0; e < VE; ++e) d[e] = m[e] == 0.f ? 0.f : d[e] * m[e];
                 }
-                stv<VE>((T*)a.dX + row * a.lddx + c0, d);
+                stv<VE>((T*)a.dX + row * a.lddx + at[i], d);
             }
         }
     }
@@ -320,8 +350,9 @@ __global__ void __launch_bounds__(1024) norm_bwd_long_kernel(const NormArgs a) {
             if (a.dS) Elem<T>::st((T*)a.dS + row * a.lddsum + c, d);
             if (a.dX) {
                 if (a.use_drop) {
-                    const float m = drop_mul64(key, a.drop.thresh, a.drop.inv_keep, row * C + c);
-                    d = m == 0.f ? 0.f : d * m;
+                    float m[1];
+                    drop_vec<1>(m, key, a.drop.thresh, a.drop.inv_keep, row * C + c);
+                    d = m[0] == 0.f ? 0.f : d * m[0];
                 }
                 Elem<T>::st((T*)a.dX + row * a.lddx + c, d);
             }
@@ -369,6 +400,11 @@ Shape shape_of(int C, int ve) {
     return s;
 }
 
+// parameters are read in vectors of min(ve, 4) floats
+int par_align(const void* p, int ve) {
+    while (ve > 1 && p && (uintptr_t)p % ((ve < 4 ? ve : 4) * 4)) ve >>= 1;
+    return ve;
+}
 int row_align(const void* p, long ld, int es, int ve) {
     while (ve > 1 && (p && (((uintptr_t)p % (uintptr_t)(ve * es)) || ld % ve))) ve >>= 1;
     return ve;
@@ -390,8 +426,15 @@ long bwd_blocks(long rows, int C, int es, int G) {
 template <typename T, int VE, int NC, int G>
 void run(const NormArgs& a, bool bwd, long nblk, hipStream_t s) {
     constexpr int NT = G > 256 ? G : 256, GPB = G > 256 ? 1 : 256 / G;
-    if (bwd) hipLaunchKernelGGL((norm_bwd_kernel<T, VE, NC, G>), dim3((unsigned)nblk), dim3(NT), 0, s, a);
-    else hipLaunchKernelGGL((norm_fwd_kernel<T, VE, NC, G>), dim3((unsigned)((a.rows + GPB - 1) / GPB)), dim3(NT), 0, s, a);
+    if (bwd) {
+        if (a.dSt) hipLaunchKernelGGL((norm_bwd_kernel<T, VE, NC, G, true>), dim3((unsigned)nblk), dim3(NT), 0, s, a);
+        else hipLaunchKernelGGL((norm_bwd_kernel<T, VE, NC, G, false>), dim3((unsigned)nblk), dim3(NT), 0, s, a);
+        return;
+    }
+    const long need = (a.rows + GPB - 1) / GPB, most = 8L * 256 * 256 / NT;       // (no more than run at once: gamma and beta are read once each)
+    const dim3 grid((unsigned)(need < most ? need : most));
+    if (a.Res) hipLaunchKernelGGL((norm_fwd_kernel<T, VE, NC, G, true>), grid, dim3(NT), 0, s, a);
+    else hipLaunchKernelGGL((norm_fwd_kernel<T, VE, NC, G, false>), grid, dim3(NT), 0, s, a);
 }
 // (only what shape_of picks is built: every NC for a wave, NC > MAXV / VE / 4 for 256 threads, the largest beyond)
 template <typename T, int VE, int NC>
@@ -435,6 +478,7 @@ extern "C" int gast_layer_norm_fwd(int dtype, const void* X, long ldx, const voi
     int ve = row_align(X, ldx, es, 16 / es);
     ve = row_align(Y, ldy, es, ve);
     if (residual) ve = row_align(S, lds, es, row_align(residual, ldr, es, ve));
+    ve = par_align(gamma, par_align(beta, ve));
     const Shape sh = shape_of(C, ve);
     NormArgs a = {};
     a.X = X; a.ldx = ldx; a.Res = residual; a.ldr = ldr; a.rows = rows; a.C = C; a.gamma = gamma; a.beta = beta; a.eps = eps;
@@ -464,6 +508,7 @@ extern "C" int gast_layer_norm_bwd(int dtype, const void* dY, long lddy, const v
     ve = row_align(dStream, ldds, es, ve);
     ve = row_align(dX, lddx, es, ve);
     ve = row_align(dS, lddsum, es, ve);
+    ve = par_align(gamma, ve);
     const Shape sh = shape_of(C, ve);
     NormArgs a = {};
     a.dY = dY; a.lddy = lddy; a.dSt = dStream; a.ldds = ldds; a.S = (void*)S; a.lds = lds; a.rows = rows; a.C = C; a.gamma = gamma;
