@@ -47,5 +47,23 @@ if [ -z "$GAST_SKIP_F16" ]; then      # (GAST_SKIP_F16=1: kernel-development bui
   build_flavour "$HERE/build/f16" "$HERE/../gast_hip/libgast_hip_f16.so" "-DGAST_H16_F16" &
   P2=$!
 fi
+# gast_hip/_temporal.so: the sequence operators as torch functions (host code; opens the two libraries by path)
+build_nodes() {
+  local SRC="$HERE/temporal_nodes.cpp" LIB="$HERE/../gast_hip/_temporal.so" STAMP="$HERE/build/temporal_nodes.sha"
+  local PY="${PYTHON:-python3}" T I want
+  T="$($PY -c 'import os, torch; print(os.path.dirname(torch.__file__))')"
+  I="$($PY -c 'import sysconfig; print(sysconfig.get_paths()["include"])')"
+  local FL="-O2 -std=c++17 -fPIC -shared -DTORCH_EXTENSION_NAME=_temporal -D__HIP_PLATFORM_AMD__ -DUSE_ROCM"
+  want="$( (echo "$FL $T $I"; cat "$T/version.py" "$SRC" "$HERE/../../include/gast_hip.h") | sha256sum | cut -d' ' -f1)"
+  if [ -f "$LIB" ] && [ "$want" = "$(cat "$STAMP" 2>/dev/null || true)" ]; then echo "built $LIB (up to date)"; return 0; fi
+  rm -f "$STAMP"
+  g++ $FL "$SRC" -I"$T/include" -I"$T/include/torch/csrc/api/include" -I"$I" -I/opt/rocm/include -L"$T/lib" -lc10 -lc10_hip -ltorch -ltorch_cpu \
+      -ltorch_python -ldl -o "$LIB" || { echo "compile failed: temporal_nodes.cpp" >&2; return 1; }
+  echo "$want" > "$STAMP"
+  echo "built $LIB"
+}
+build_nodes &
+P3=$!
 wait $P1 || exit 1
 if [ -n "$P2" ]; then wait $P2 || exit 1; fi
+wait $P3 || exit 1

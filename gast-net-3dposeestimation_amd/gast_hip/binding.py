@@ -129,25 +129,6 @@ class _BnBwdJob(C.Structure):
     _fields_ = [('f', _BnBwdFinJob), ('dz', C.c_void_p), ('lddz', C.c_int), ('X', C.c_void_p), ('ldx', C.c_int), ('rows', C.c_long)]
 
 
-class Seq(C.Structure):
-    """gast_seq: a (B, T, J, H, D) view, D contiguous"""
-    _fields_ = [('p', C.c_void_p), ('b', C.c_long), ('t', C.c_long), ('j', C.c_long), ('h', C.c_long)]
-
-
-ROTARY_MAX_BATCH, ROTARY_MAX_D, DECAY_MAX_D = 4, 1024, 128
-
-
-class _RotaryJob(C.Structure):
-    _fields_ = [('x', Seq), ('y', Seq), ('H', C.c_int)]
-
-
-class _DecayArgs(C.Structure):
-    _fields_ = [('dtype', C.c_int), ('B', C.c_int), ('T', C.c_int), ('J', C.c_int), ('H', C.c_int), ('Dk', C.c_int), ('Dv', C.c_int),
-                ('scale', C.c_float), ('log_decay', C.c_void_p), ('lengths', C.c_void_p), ('q', Seq), ('k', Seq), ('v', Seq), ('o', Seq),
-                ('state', C.c_void_p), ('state_out', C.c_void_p), ('d_o', Seq), ('dq', Seq), ('dk', Seq), ('dv', Seq),
-                ('dstate_out', C.c_void_p), ('dstate', C.c_void_p), ('ws', C.c_void_p)]
-
-
 # The library exists in two 16-bit STORAGE flavours built from the same sources (csrc/build.sh, csrc/common.h): libgast_hip.so keeps
 # GAST_BF16 tensors as bfloat16, libgast_hip_f16.so as IEEE binary16 (GAST_HIP_DTYPE=f16).  Same ABI; the process-wide flavour
 # (`set_h16`, per thread) decides which one the op set calls and which 16-bit torch dtype `_dt` accepts -- a tensor of the other kind raises.
@@ -190,14 +171,18 @@ def h16_dtype():
     return _H16['dtype']
 
 
+def library_path(h16):
+    if h16 != torch.float16 and os.environ.get('GAST_HIP_LIB_EXPERIMENT'):      # kernel A/B builds (scripts/): a sibling library by suffix
+        return os.path.join(_HERE, 'libgast_hip_%s.so' % os.environ['GAST_HIP_LIB_EXPERIMENT'])
+    return LIB_PATH_F16 if h16 == torch.float16 else LIB_PATH
+
+
 def load_library(h16=torch.bfloat16):
     """Load libgast_hip.so (or its binary16 flavour) or raise -- the HIP path is the only path."""
     lib = _libs.get(h16)
     if lib is not None:
         return lib
-    path = LIB_PATH_F16 if h16 == torch.float16 else LIB_PATH
-    if h16 != torch.float16 and os.environ.get('GAST_HIP_LIB_EXPERIMENT'):      # kernel A/B builds (scripts/): a sibling library by suffix
-        path = os.path.join(_HERE, 'libgast_hip_%s.so' % os.environ['GAST_HIP_LIB_EXPERIMENT'])
+    path = library_path(h16)
     if not os.path.exists(path):
         raise RuntimeError('gast_hip: %s not found -- build it with `python -c "import __graft_entry__ as g; g.build()"` '
                            '(hipcc --offload-arch=gfx950). There is no CPU/PyTorch fallback.' % path)
@@ -266,14 +251,15 @@ def load_library(h16=torch.bfloat16):
         'gast_prep': [C.POINTER(_PrepArgs), vp],
         'gast_chunk_gather': [vp, vp, vp, vp, vp, cl, ci, ci, ci, ci, ci, ci, ci, ci, ci, vp, vp, vp, vp, vp, vp],
         'gast_stream_shift_multi': [C.POINTER(_StreamShiftJob), ci, vp],
-        'gast_rotary_multi': [ci, C.POINTER(_RotaryJob), ci, ci, ci, ci, ci, ci, ci, vp, ci, cl, cl, vp, cf, ci, vp],
+        # (the sequence operators are called from gast_hip/_temporal.so, csrc/temporal_nodes.cpp)
+        'gast_rotary_multi': [ci, vp, ci, ci, ci, ci, ci, ci, ci, vp, ci, cl, cl, vp, cf, ci, vp],
         'gast_layer_norm_fwd': [ci, vp, cl, vp, cl, cl, ci, vp, vp, cf, ci, cu, _Dropout, vp, cl, vp, cl, vp, vp, vp],
         'gast_layer_norm_bwd': [ci, vp, cl, vp, cl, vp, cl, cl, ci, vp, vp, vp, ci, cu, _Dropout, vp, cl, vp, cl, vp, vp, vp, vp],
         'gast_layer_norm_bwd_ws_floats': [cl, ci],
-        'gast_decay_fwd': [C.POINTER(_DecayArgs), vp],
-        'gast_decay_bwd': [C.POINTER(_DecayArgs), vp],
+        'gast_decay_fwd': [vp, vp],
+        'gast_decay_bwd': [vp, vp],
         'gast_decay_ws_floats': [ci, ci, ci, ci, ci, ci, ci],
-        'gast_decay_step': [C.POINTER(_DecayArgs), vp],
+        'gast_decay_step': [vp, vp],
     }
     for name, argtypes in sig.items():
         fn = getattr(lib, name)
@@ -318,12 +304,6 @@ def _ld(t):
     if t.dim() != 2 or t.stride(1) != 1:
         raise RuntimeError('gast_hip: expected a 2-D row-major view, got shape %s strides %s' % (tuple(t.shape), t.stride()))
     return t.stride(0)
-
-
-def seq(t):
-    """gast_seq of a (B, T, J, H, D) tensor whose D values are contiguous"""
-    s = t.stride()
-    return Seq(t.data_ptr(), s[0], s[1], s[2], s[3])
 
 
 def _dt(t):
@@ -1007,85 +987,6 @@ class HipOps:
                 a.B, a.Tb, a.X, a.ldnew = int(buf.shape[0]), int(buf.shape[1]), int(buf.shape[2]), int(newest.stride(0))
             self.launches += 1
             _check(self.lib.gast_stream_shift_multi(arr, len(chunk), _stream()), 'gast_stream_shift_multi')
-
-    # -- sequence operators (gast_hip/temporal.py, which checks shapes).  The flavour of the library goes by the tensors' own type.
-    @staticmethod
-    def _typed(t):
-        if t.dtype == torch.float32:
-            return load_library(), GAST_F32
-        return load_library(t.dtype), GAST_BF16
-
-    def rotary_multi(self, pairs, positions, freqs, R, interleaved, scale, backward):
-        """pairs: (x, y) views (B, T, J, H, D) with B, T, J, D in common; positions (B or 1, T) int32 / int64; freqs (R / 2,) float64"""
-        x0 = pairs[0][0]
-        B, T, J, _, D = x0.shape
-        lib, dt = self._typed(x0)
-        jobs = (_RotaryJob * len(pairs))()
-        for a, (x, y) in zip(jobs, pairs):
-            a.x, a.y, a.H = seq(x), seq(y), x.shape[3]
-        self.launches += 1
-        _check(lib.gast_rotary_multi(dt, jobs, len(pairs), B, T, J, D, R, int(interleaved), positions.data_ptr(),
-                                     int(positions.dtype == torch.int64), positions.stride(0) if positions.shape[0] > 1 else 0,
-                                     positions.stride(1), freqs.data_ptr(), scale, int(backward), _stream()), 'gast_rotary_multi')
-
-    def layer_norm_fwd(self, X, residual, gamma, beta, eps, drop, salt, S, Y, mean, rstd):
-        lib, dt = self._typed(X)
-        self.launches += 1
-        _check(lib.gast_layer_norm_fwd(dt, _p(X), X.stride(0), _p(residual), 0 if residual is None else residual.stride(0), X.shape[0], X.shape[1],
-                                       _p(gamma), _p(beta), eps, int(drop is not None), salt, _drop(drop), _p(S), 0 if S is None else S.stride(0),
-                                       _p(Y), Y.stride(0), _p(mean), _p(rstd), _stream()), 'gast_layer_norm_fwd')
-
-    def layer_norm_bwd(self, dY, dStream, S, gamma, mean, rstd, drop, salt, dX, dS, dgamma, dbeta):
-        lib, dt = self._typed(S)
-        rows, C_ = S.shape
-        ws = None
-        if dgamma is not None or dbeta is not None:
-            ws = torch.empty(lib.gast_layer_norm_bwd_ws_floats(rows, C_), dtype=torch.float32, device=S.device)
-        ld = [0 if t is None else t.stride(0) for t in (dY, dStream, dX, dS)]
-        self.launches += 1 if ws is None else 2
-        _check(lib.gast_layer_norm_bwd(dt, _p(dY), ld[0], _p(dStream), ld[1], _p(S), S.stride(0), rows, C_, _p(gamma), _p(mean), _p(rstd),
-                                       int(drop is not None), salt, _drop(drop), _p(dX), ld[2], _p(dS), ld[3], _p(dgamma), _p(dbeta), _p(ws),
-                                       _stream()), 'gast_layer_norm_bwd')
-
-    def _decay_args(self, q, k, v, log_decay, lengths, scale, state):
-        a = _DecayArgs()
-        a.B, a.T, a.J, a.H, a.Dk = q.shape
-        a.Dv = v.shape[4]
-        a.scale = scale
-        a.log_decay, a.lengths, a.state = log_decay.data_ptr(), _p(lengths), _p(state)
-        a.q, a.k, a.v = seq(q), seq(k), seq(v)
-        return a
-
-    def _decay_ws(self, lib, a, dev, backward):
-        n = lib.gast_decay_ws_floats(a.B, a.T, a.J, a.H, a.Dk, a.Dv, backward)
-        return torch.empty(n, dtype=torch.float32, device=dev) if n else None
-
-    def decay_fwd(self, q, k, v, log_decay, lengths, scale, state, o, state_out):
-        lib, dt = self._typed(q)
-        a = self._decay_args(q, k, v, log_decay, lengths, scale, state)
-        a.dtype, a.o, a.state_out = dt, seq(o), _p(state_out)
-        ws = self._decay_ws(lib, a, q.device, 0)
-        a.ws = _p(ws)
-        self.launches += 1
-        _check(lib.gast_decay_fwd(C.byref(a), _stream()), 'gast_decay_fwd')
-
-    def decay_bwd(self, q, k, v, log_decay, lengths, scale, state, d_o, dstate_out, dq, dk, dv, dstate):
-        lib, dt = self._typed(q)
-        a = self._decay_args(q, k, v, log_decay, lengths, scale, state)
-        a.dtype, a.d_o, a.dq, a.dk, a.dv = dt, seq(d_o), seq(dq), seq(dk), seq(dv)
-        a.dstate_out, a.dstate = _p(dstate_out), _p(dstate)
-        ws = self._decay_ws(lib, a, q.device, 1)
-        a.ws = _p(ws)
-        self.launches += 1
-        _check(lib.gast_decay_bwd(C.byref(a), _stream()), 'gast_decay_bwd')
-
-    def decay_step(self, q, k, v, log_decay, lengths, scale, state, o):
-        """q, k, v, o: views with T = 1; state is updated in place"""
-        lib, dt = self._typed(q)
-        a = self._decay_args(q, k, v, log_decay, lengths, scale, state)
-        a.dtype, a.o = dt, seq(o)
-        self.launches += 1
-        _check(lib.gast_decay_step(C.byref(a), _stream()), 'gast_decay_step')
 
     def prep(self, zero, seed=None, pad=None):
         """Pass prologue (gast_prep): zero-fill the tensors of `zero` (contiguous device tensors), seed = (counter, per-pass copy):

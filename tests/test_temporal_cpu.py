@@ -122,3 +122,4 @@ def test_the_oracles_recurrence_is_the_sum_over_earlier_tokens():
     a = torch.einsum('bthd,bshd->bhts', q[:, :, 0], k[:, :, 0]) * w * 0.5
     assert torch.allclose(o[:, :, 0], torch.einsum('bhts,bshe->bthe', a, v[:, :, 0]), rtol=1e-12, atol=1e-12)
     assert torch.allclose(S[:, 0], torch.einsum('bshd,hs,bshe->bhde', k[:, :, 0], torch.exp(ld[:, None] * (8 - t)), v[:, :, 0]), rtol=1e-12, atol=1e-12)
+
