@@ -219,8 +219,8 @@ gast_decay_args decay_args(const Tensor& q, const Tensor& k, const Tensor& v, co
     a.state = f32(state);
     return a;
 }
-Tensor decay_ws(const Lib& l, gast_decay_args& a, const Tensor& like, int backward) {
-    const long n = l.decay_ws(a.B, a.T, a.J, a.H, a.Dk, a.Dv, backward);
+Tensor decay_ws(const Lib& l, gast_decay_args& a, const Tensor& like) {
+    const long n = l.decay_ws(a.dtype, a.B, a.T, a.J, a.H, a.Dk, a.Dv);
     Tensor ws;
     if (n) ws = floats(like, {n});
     a.ws = f32(ws);
@@ -228,7 +228,7 @@ Tensor decay_ws(const Lib& l, gast_decay_args& a, const Tensor& like, int backwa
 }
 
 variable_list decay_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, const Tensor& state, const Tensor& lengths,
-                            double scale, bool want_state) {
+                            double scale, bool want_state, Tensor* segments = nullptr) {
     const Tensor o = fresh(v);
     Tensor next;
     if (want_state) next = floats(q, {q.size(0), q.size(2), q.size(3), q.size(4), v.size(4)});
@@ -238,8 +238,9 @@ variable_list decay_forward(const Tensor& q, const Tensor& k, const Tensor& v, c
         gast_decay_args a = decay_args(q, k, v, log_decay, state, lengths, scale);
         a.o = seq(o);
         a.state_out = f32(next);
-        const Tensor ws = decay_ws(l, a, q, 0);
+        const Tensor ws = decay_ws(l, a, q);
         done(l.decay_fwd(&a, here.stream), "gast_decay_fwd");
+        if (segments) *segments = ws;
     } else if (want_state) {
         if (state.defined()) next.copy_(state);
         else next.zero_();
@@ -251,10 +252,12 @@ struct DecayNode : torch::autograd::Function<DecayNode> {
     static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay,
                                  const optional<Tensor>& state_, const optional<Tensor>& lengths_, double scale, bool want_state) {
         const Tensor state = or_none(state_), lengths = or_none(lengths_);
-        ctx->save_for_backward({q, k, v, log_decay, state, lengths});
+        Tensor segments;                                   // the states before the segments of a long sequence: the backward pass wants them again
+        variable_list out = decay_forward(q, k, v, log_decay, state, lengths, scale, want_state, &segments);
+        ctx->save_for_backward({q, k, v, log_decay, state, lengths, segments});
         ctx->saved_data["scale"] = scale;
         ctx->set_materialize_grads(false);
-        return decay_forward(q, k, v, log_decay, state, lengths, scale, want_state);
+        return out;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const auto s = ctx->get_saved_variables();
@@ -271,7 +274,8 @@ struct DecayNode : torch::autograd::Function<DecayNode> {
             a.d_o = seq(d_o); a.dq = seq(dq); a.dk = seq(dk); a.dv = seq(dv);
             a.dstate_out = f32(dnext);
             a.dstate = f32(dstate);
-            const Tensor ws = decay_ws(l, a, q, 1);
+            const Tensor ws = decay_ws(l, a, q);
+            a.ws_fwd = f32(s[6]);
             done(l.decay_bwd(&a, here.stream), "gast_decay_bwd");
         } else if (dstate.defined()) {
             if (dnext.defined()) dstate.copy_(dnext);

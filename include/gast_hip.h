@@ -541,11 +541,12 @@ typedef struct {
     gast_seq d_o, dq, dk, dv;
     const float* dstate_out;
     float* dstate;
-    float* ws;                   /* gast_decay_ws_floats() floats (null where that is 0) */
+    float* ws;                   /* gast_decay_ws_floats() floats (null where that is 0; backward without ws_fwd: twice as many) */
+    const float* ws_fwd;         /* backward: what gast_decay_fwd left in its ws for the same q, k, v, log_decay, lengths and state, or null */
 } gast_decay_args;
 int gast_decay_fwd(const gast_decay_args* args, gast_stream_t stream);
 int gast_decay_bwd(const gast_decay_args* args, gast_stream_t stream);
-long gast_decay_ws_floats(int B, int T, int J, int H, int Dk, int Dv, int backward);
+long gast_decay_ws_floats(int dtype, int B, int T, int J, int H, int Dk, int Dv);
 /* One token of every stream: T = 1, state updated in place (state_out is ignored); streams with lengths[b] < 1 keep their state, o = 0. */
 int gast_decay_step(const gast_decay_args* args, gast_stream_t stream);
 
