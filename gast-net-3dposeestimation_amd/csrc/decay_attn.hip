@@ -113,8 +113,7 @@ __device__ __forceinline__ Split stored_parts(const Frag<bf16_t>& f) {
     unpack(f, v);
     return split16(v);
 }
-template <typename V> __device__ __forceinline__ void mma_fs(f32x16& c, const V& av, const Frag<bf16_t>& b) {
-    const Split a = split16(av);
+__device__ __forceinline__ void mma_fs(f32x16& c, const Split& a, const Frag<bf16_t>& b) {
 #ifdef GAST_H16_F16
     const Split p = stored_parts(b);
 #pragma unroll
@@ -208,14 +207,52 @@ template <int G> __device__ __forceinline__ void mma_into(f32x16 (&X)[G], const 
 template <typename T> struct Prepared;
 template <> struct Prepared<float> {
     float v[16];
-    __device__ __forceinline__ void set(const float (&x)[16]) {
+    template <typename V> __device__ __forceinline__ void set(const V& x) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) v[i] = x[i];
     }
 };
-template <> struct Prepared<bf16_t> { Split v; __device__ __forceinline__ void set(const float (&x)[16]) { v = split16(x); } };
+template <> struct Prepared<bf16_t> { Split v; template <typename V> __device__ __forceinline__ void set(const V& x) { v = split16(x); } };
 template <typename T> struct Exact : Prepared<float> {};
 template <> struct Exact<bf16_t> { Parts v; __device__ __forceinline__ void set(const float (&x)[16]) { v = parts16(x); } };
+
+// Infinities and NaN among stored values: where they are zeros, and ones where they are (everything else zero)
+__device__ __forceinline__ bool any_wild(const Frag<float>& f) {
+    float t = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) t = fmaf(f.x[i], 0.f, t);
+    return t != 0.f;
+}
+__device__ __forceinline__ void part_wild(const Frag<float>& f, Frag<float>& tame, Frag<float>& wild) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const bool w = !(fabsf(f.x[i]) < INFINITY);
+        tame.x[i] = w ? 0.f : f.x[i];
+        wild.x[i] = w ? 1.f : 0.f;
+    }
+}
+// (16 bits: an exponent of all ones carries into the sign's place)
+#ifdef GAST_H16_F16
+constexpr uint32_t H_CARRY = 0x04000400u, H_ONE = 0x3c003c00u;
+#else
+constexpr uint32_t H_CARRY = 0x00800080u, H_ONE = 0x3f803f80u;
+#endif
+__device__ __forceinline__ uint32_t wild2(uint32_t x) { return ((x & 0x7fff7fffu) + H_CARRY) & 0x80008000u; }
+__device__ __forceinline__ bool any_wild(const Frag<bf16_t>& f) {
+    return (wild2(f.x[0].x) | wild2(f.x[0].y) | wild2(f.x[0].z) | wild2(f.x[0].w) | wild2(f.x[1].x) | wild2(f.x[1].y) | wild2(f.x[1].z) | wild2(f.x[1].w)) != 0;
+}
+__device__ __forceinline__ void part_wild2(uint32_t x, uint32_t& tame, uint32_t& wild) {
+    const uint32_t w = (wild2(x) >> 15) * 0xffffu;
+    tame = x & ~w;
+    wild = H_ONE & w;
+}
+__device__ __forceinline__ void part_wild(const Frag<bf16_t>& f, Frag<bf16_t>& tame, Frag<bf16_t>& wild) {
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        part_wild2(f.x[q].x, tame.x[q].x, wild.x[q].x); part_wild2(f.x[q].y, tame.x[q].y, wild.x[q].y);
+        part_wild2(f.x[q].z, tame.x[q].z, wild.x[q].z); part_wild2(f.x[q].w, tame.x[q].w, wild.x[q].w);
+    }
+}
 
 // The 32 x DP tokens of one tensor on their way from memory to LDS: 16 elements a thread of NW waves.  16 bits: 8 channels of two rows,
 // so that a turned word holds both; four lanes read 64 contiguous bytes and the turned words of a wave fall into 64 different banks.
@@ -302,10 +339,23 @@ __device__ __forceinline__ void bring_odd(Stage<T>& s, const View& v, int t0, in
     }
 }
 
-// Y (32 columns of out by 32 tokens, the token in lane % 32) to memory by way of LDS, so that a row leaves in 16-byte pieces
-template <typename T>
-__device__ __forceinline__ void put_tile(const f32x16& Y, T* tile, T* O, long st, int t0, int n, int c0, int D, int al, int lane) {
-    constexpr int VE = 16 / sizeof(T), VR = 32 / VE;      // vectors of a row
+// Y (32 columns of out by 32 tokens, the token in lane % 32) to memory.  fp32: four registers are 16 bytes of a row, and go out as they are.
+__device__ __forceinline__ void put_tile(const f32x16& Y, float*, float* O, long st, int t0, int n, int c0, int D, int al, int lane) {
+    const int row = lane & 31;
+    float* p = O + (long)(t0 + row) * st + c0 + 4 * (lane >> 5);
+    const int left = D - c0 - 4 * (lane >> 5);
+    if (row >= n) return;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        if (al && 8 * q + 4 <= left) *(float4*)(p + 8 * q) = make_float4(Y[4 * q], Y[4 * q + 1], Y[4 * q + 2], Y[4 * q + 3]);
+        else
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (8 * q + e < left) p[8 * q + e] = Y[4 * q + e];
+    }
+}
+// 16 bits: by way of LDS, so that a row leaves in 16-byte pieces
+__device__ __forceinline__ void put_tile(const f32x16& Y, bf16_t* tile, bf16_t* O, long st, int t0, int n, int c0, int D, int al, int lane) {
 #pragma unroll
     for (int q = 0; q < 4; ++q)
         st4(tile + (lane & 31) * TS + 8 * q + 4 * (lane >> 5), make_float4(Y[4 * q], Y[4 * q + 1], Y[4 * q + 2], Y[4 * q + 3]));
@@ -313,16 +363,16 @@ __device__ __forceinline__ void put_tile(const f32x16& Y, T* tile, T* O, long st
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 #pragma unroll
-    for (int k = 0; k < VR / 2; ++k) {
-        const int row = lane / VR + k * (64 / VR), e = (lane % VR) * VE;
+    for (int k = 0; k < 2; ++k) {
+        const int row = lane / 4 + 16 * k, e = (lane % 4) * 8;
         if (row >= n || c0 + e >= D) continue;
-        const T* s = tile + row * TS + e;
-        T* p = O + (long)(t0 + row) * st + c0 + e;
-        if (al && c0 + e + VE <= D) {
-            const uint2 u = *(const uint2*)s, w = *(const uint2*)(s + VE / 2);
+        const bf16_t* s = tile + row * TS + e;
+        bf16_t* p = O + (long)(t0 + row) * st + c0 + e;
+        if (al && c0 + e + 8 <= D) {
+            const uint2 u = *(const uint2*)s, w = *(const uint2*)(s + 4);
             *(uint4*)p = make_uint4(u.x, u.y, w.x, w.y);
         } else {
-            for (int x = 0; x < VE && c0 + e + x < D; ++x) p[x] = s[x];
+            for (int x = 0; x < 8 && c0 + e + x < D; ++x) p[x] = s[x];
         }
     }
 }
@@ -365,12 +415,12 @@ struct ChunkArgs {
     int B, T, J, H, nseg, L, skip_last;     // segments of L tokens; skip_last: nobody reads the sums of the last one in this direction
 };
 
-// LDS of a kernel, in elements: tiles as rows, turned tiles, output tiles of the waves (ONE: over the wave's own columns of c)
+// LDS of a kernel, in elements: tiles as rows, turned tiles, output tiles of the waves (ONE: over the wave's own columns of c; fp32: none)
 template <int DP, int MODE> struct Lay {
     static constexpr int NW = DP / 32, RS = DP + 4, ROWS = CT * RS, TURN = DP * TS;
     static constexpr int GROUPS = MODE == TWO ? 2 : MODE == THREE ? 3 : 1, NT = GROUPS * NW * 64;
     static constexpr int NROWS = MODE == ONE ? 2 : MODE == SUMS ? 0 : 4, NTURN = MODE == THREE ? 3 : 2;
-    static constexpr int OUT = MODE == TWO || MODE == THREE ? GROUPS * NW * 32 * TS : 0, TILES = NROWS * ROWS + NTURN * TURN;
+    static constexpr int TILES = NROWS * ROWS + NTURN * TURN;
 };
 
 // exp(g n) to two steps of fp32, however long n is: the product's rounding is carried along
@@ -388,10 +438,11 @@ struct Powers {
 };
 template <typename T, int DP, int MODE, bool STATE> struct Lds {
     using L = Lay<DP, MODE>;
+    static constexpr int OUT = sizeof(T) == 2 && (MODE == TWO || MODE == THREE) ? L::NT / 64 * 32 * TS : 0;
     // two sets of tiles (one barrier a chunk instead of two) where the waves that the registers allow still fit: 20 KB a wave
-    static constexpr int NBUF = STATE && 2 * L::TILES * (int)sizeof(T) + L::OUT * (int)sizeof(T) <= 20 * 1024 * L::GROUPS * L::NW ? 2 : 1;
+    static constexpr int NBUF = STATE && (2 * L::TILES + OUT) * (int)sizeof(T) <= 20 * 1024 * L::GROUPS * L::NW ? 2 : 1;
     Powers pw;
-    T tiles[NBUF * L::TILES + L::OUT];
+    T tiles[NBUF * L::TILES + OUT];
 };
 
 
@@ -455,13 +506,16 @@ __global__ void __launch_bounds__((Lay<DP, MODE>::NT), 2) chunk_kernel(const Chu
     if (nchunk) fetch(c_first);
     Powers& pw = m.pw;
     if (tid <= CT) {
-        const float p = power(lg, (float)tid), u = power(lg, 32.f * tid);
+        const float p = power(lg, (float)tid);
         pw.up[tid] = p;
-        pw.unit[tid] = u;
-        pw.per_unit[tid] = 1.f / u;
-        if (tid < CT) {
-            pw.down[CT - 1 - tid] = p;
-            pw.down[CT + tid] = 0.f;
+        if constexpr (STATE) {
+            const float u = power(lg, 32.f * tid);
+            pw.unit[tid] = u;
+            pw.per_unit[tid] = 1.f / u;
+            if (tid < CT) {
+                pw.down[CT - 1 - tid] = p;
+                pw.down[CT + tid] = 0.f;
+            }
         }
     }
     const float steps = 5.545f / (32.f * fabsf(lg));       // ln 2^8
@@ -505,18 +559,14 @@ __global__ void __launch_bounds__((Lay<DP, MODE>::NT), 2) chunk_kernel(const Chu
         if (works) {
             const T *ta = tiles + oa + col * RS, *tb = tiles + ob + col * RS, *tbT = tiles + obT + col * TS;
             T* const tc = tiles + oc;
-            // ---- P[j][i] = b_j a_i, Y[e][i] = sum_d X[d][e] a_i[d]; meanwhile c as it enters the state
+            // ---- P[j][i] = b_j a_i, Y[e][i] = sum_d X[d][e] a_i[d].  What one step's products need is read and split during the step before.
             f32x16 P = {}, Y = {};
-            if constexpr (MODE != SUMS)
-#pragma unroll
-                for (int q = 0; q < G; ++q) {
-                    const Frag<T> fa = ld_frag(ta + 32 * q, half), fb = ld_frag(tb + 32 * q, half);
-                    mma(P, fb, fa);
-                    if constexpr (STATE) mma_fs(Y, X[q], fa);
-                }
             const Frag<T> fc = ld_frag(tc + col * TS, half);
+            Frag<T> fk[G];
             Exact<T> pv;
-            if constexpr (STATE) {
+            auto enter = [&] {                             // c as it enters the state, and the other side of that product
+#pragma unroll
+                for (int q = 0; q < G; ++q) fk[q] = ld_frag(tbT + 32 * q * TS, half);
                 float v[16];
                 unpack(fc, v);
                 const float w = ro.fk * pw.per_unit[pa];
@@ -524,19 +574,33 @@ __global__ void __launch_bounds__((Lay<DP, MODE>::NT), 2) chunk_kernel(const Chu
 #pragma unroll
                 for (int r = 0; r < 16; ++r) v[r] *= in_by[8 * (r >> 2) + (r & 3)] * w;
                 pv.set(v);
+            };
+            if constexpr (MODE != SUMS) {
+                Frag<T> fa = ld_frag(ta, half), fb = ld_frag(tb, half), na = fa, nb = fb;
+                Prepared<T> px, nx;
+                if constexpr (STATE) px.set(X[0]);
+#pragma unroll
+                for (int q = 0; q < G; ++q) {
+                    if (q + 1 < G) na = ld_frag(ta + 32 * (q + 1), half), nb = ld_frag(tb + 32 * (q + 1), half);
+                    mma(P, fb, fa);
+                    if constexpr (STATE) {
+                        mma_fs(Y, px.v, fa);
+                        if (q + 1 < G) nx.set(X[q + 1]);
+                        else enter();
+                    }
+                    fa = na; fb = nb; px = nx;
+                }
+            } else {
+                enter();
+            }
+            if constexpr (STATE)
                 if (renew) {
                     const float f = pw.unit[p] * pw.up[steps_on];
 #pragma unroll
                     for (int q = 0; q < G; ++q) X[q] *= f;
                 }
-            }
             // ---- X += b c; meanwhile the scores, and Y[e][i] += sum_j c_j[e] P[j][i]
-            if constexpr (STATE) {
-                Frag<T> fk[G];
-#pragma unroll
-                for (int q = 0; q < G; ++q) fk[q] = ld_frag(tbT + 32 * q * TS, half);
-                mma_into<G>(X, fk, pv.v);
-            }
+            if constexpr (STATE) mma_into<G>(X, fk, pv.v);
             if constexpr (MODE != SUMS) {
                 float sc[16];
 #pragma unroll
@@ -544,8 +608,32 @@ __global__ void __launch_bounds__((Lay<DP, MODE>::NT), 2) chunk_kernel(const Chu
                 Prepared<T> pp;
                 pp.set(sc);
                 if constexpr (STATE) Y *= pw.up[max((rev ? n - 1 - col : col) + 1 - first, 0)] * pw.unit[p] * ro.fo;
-                mma_sf(Y, fc, pp.v);
-                put_tile<T>(Y, BWD ? m.tiles + NBUF * L::TILES + wave * 32 * TS : tc, O, ro.out.t, t0, n, wv * 32, D2, ro.al, lane);
+                // A score of zero is no mask for an infinity or NaN of a token that i does not see: those chunks are worked on with zeros in
+                // their place, and only outputs that see one of them take the product as it is.  (One that enters the state is seen there.)
+                bool wild;
+                if constexpr (STATE) wild = !(fabsf(X[0][0]) < INFINITY);
+                else wild = any_wild(fc);
+                if (__any(wild)) {
+                    Frag<T> tame, ones;
+                    part_wild(fc, tame, ones);
+                    f32x16 Z = {};
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) sc[r] = (8 * (r >> 2) + 4 * half + (r & 3) - col) * (rev ? 1 : -1) >= 0 ? 1.f : 0.f;
+                    Prepared<T> sees;
+                    sees.set(sc);
+                    mma_sf(Z, ones, sees.v);
+                    uint32_t at = 0;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) at |= Z[r] != 0.f ? 1u << r : 0u;
+                    Z = Y;
+                    mma_sf(Z, tame, pp.v);
+                    mma_sf(Y, fc, pp.v);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) Y[r] = at >> r & 1 ? Y[r] : Z[r];
+                } else {
+                    mma_sf(Y, fc, pp.v);
+                }
+                put_tile(Y, BWD ? m.tiles + NBUF * L::TILES + wave * 32 * TS : tc, O, ro.out.t, t0, n, wv * 32, D2, ro.al, lane);
             }
         }
         if constexpr (STATE) {
@@ -632,7 +720,10 @@ __global__ void __launch_bounds__(256) step_kernel(const gast_decay_args p) {
         sk[d] = Elem<T>::ld(K + d);
     }
     __syncthreads();
-    const float lam = expf(p.log_decay[h]);
+    // a lambda near 1 takes effect as lambda - 1: rounded itself, it would be off the same way at every token (10^4 tokens: 2^-11 of a state)
+    const float lg = p.log_decay[h];
+    const bool near = fabsf(lg) < 0.6931f;
+    const float f = near ? expm1f(lg) : expf(lg);
     const int rows = 256 / nv, c = tid % nv, r0 = tid / nv;
     float* S = (float*)p.state + hd * Dk * Dv + c * VE;
     float o[VE], v[VE];
@@ -647,7 +738,7 @@ __global__ void __launch_bounds__(256) step_kernel(const gast_decay_args p) {
             ldv<VE>(x, S + d * Dv);
 #pragma unroll
             for (int i = 0; i < VE; ++i) {
-                x[i] = fmaf(sk[d], v[i], lam * x[i]);
+                x[i] = fmaf(f, x[i], fmaf(sk[d], v[i], near ? x[i] : 0.f));
                 o[i] = fmaf(sq[d], x[i], o[i]);
             }
             stv<VE>(S + d * Dv, x);

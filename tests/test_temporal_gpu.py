@@ -230,6 +230,48 @@ def test_decay_long(tp, dt):
     check_decay(tp, decay_case(8, dt, 2, 1500, 1, 1, 64, 64, ragged=True, decays=[-0.001]))
 
 
+WILD = [(20, 32, [(7, 'nan'), (19, 'inf')]), (27, 64, [(13, '-inf')]), (32, 96, [(0, 'inf'), (31, 'nan')]), (200, 48, [(40, 'inf'), (170, 'nan')]), (130, 128, [(96, 'nan')]),
+        (3000, 64, [(1500, 'nan')])]
+
+
+@pytest.mark.parametrize('dt', TYPES, ids=IDS)
+@pytest.mark.parametrize('state', [False, True], ids=['fresh', 'going on'])
+@pytest.mark.parametrize('T,D,at', WILD, ids=['T%d D%d' % w[:2] for w in WILD])
+def test_decay_infinities_and_nan_reach_only_what_sees_them(tp, dt, state, T, D, at):
+    """What stands at a later token (for gradients: at an earlier one) of the sequence does not count as zero times itself.  Everything that
+    does not see a token is, to the bit, what it is with a zero there."""
+    base = decay_case(T + D, dt, 2, T, 1, 2, D, D, state=state, decays=[0.0, -0.01])
+    B, H = 2, 2
+    t = torch.arange(T)
+
+    def run(c):
+        q, k, v, s = (None if c[n] is None else c[n].cuda().requires_grad_(True) for n in ('q', 'k', 'v', 'state'))
+        o = tp.decay_attention(q, k, v, c['log_decay'].cuda(), state=s)
+        return dict(zip(('o', 'dq', 'dk', 'dv'), (o.detach(),) + torch.autograd.grad(o, (q, k, v), c['do'].cuda())))
+
+    # whose token (c), and what it reaches: its own channel e of one tensor and every channel of another, later ('+') or earlier ('-'), and
+    # every channel of its own token in a third
+    reach = dict(v=(('o', '+'), ('dq', '+'), 'dk'), k=(('dq', '+'), ('o', '+'), 'dv'), do=(('dv', '-'), ('dk', '-'), 'dq'), q=(('dk', '-'), ('dv', '-'), 'o'))
+    for name, (own, every, alone) in reach.items():
+        c, zero = dict(base), dict(base)
+        c[name], zero[name] = base[name].clone(), base[name].clone()
+        e = 5 % D
+        for token, value in at:
+            c[name][1, token, 0, 1, e] = float(value)
+            zero[name][1, token, 0, 1, e] = 0.0
+        got, want = run(c), run(zero)
+        hit = {n: torch.zeros(B, T, 1, H, D, dtype=torch.bool) for n in got}
+        for token, _ in at:
+            for (n, way), chan in ((own, slice(e, e + 1)), (every, slice(None))):
+                sees = t >= token if way == '+' else t <= token
+                hit[n][1, sees, 0, 1, chan] = True
+            hit[alone][1, token, 0, 1, :] = True
+        for n in got:
+            g, w, h = got[n].cpu(), want[n].cpu(), hit[n]
+            assert torch.equal(g[~h], w[~h]), (name, n)
+            assert not torch.isfinite(g[h]).any(), (name, n)
+
+
 @pytest.mark.parametrize('dt', TYPES, ids=IDS)
 def test_decay_reads_views(tp, dt):
     g = gen(11)
@@ -619,6 +661,62 @@ def test_two_streams_at_once(tp):
             torch.cuda.synchronize()
             for g, w in zip(got, want):
                 assert all(torch.equal(x, y) for x, y in zip(g, w))
+
+
+def test_offsets_that_pass_32_bits(tp):
+    """tokens, rows and states further than 2^32 bytes and 2^31 elements from the first one"""
+    g = gen(61)
+    dt, T, H, D = torch.bfloat16, 40, 2, 16
+    c = decay_case(61, dt, 1, T, 1, H, D, D)
+    far = torch.empty(T, 2 ** 26, dtype=dt, device='cuda')                # a token every 2^27 bytes
+    views = {}
+    for i, n in enumerate(('q', 'k', 'v', 'do')):
+        views[n] = far[:, i * 64:i * 64 + H * D].view(1, T, 1, H, D)
+        views[n].copy_(c[n])
+    check_decay(tp, c, views={n: t.detach() for n, t in views.items()})
+    pos, f = torch.arange(T).view(1, T), tp.rotary_frequencies(D)
+    close(tp.rotary(views['q'].detach(), pos.cuda(), f.cuda()), *rotary_tol(c['q'], pos, f, False, 1.0, dt), 'rotary')
+    del far, views
+    # 2^31 elements and more
+    rows, C = 2 ** 19 + 3, 4096
+    x = torch.zeros(rows, C, dtype=dt, device='cuda')
+    tail = randn(g, dt, 5, C)
+    x[-5:] = tail.cuda()
+    x.requires_grad_(True)
+    y = tp.layer_norm(x)
+    tols = norm_tols(tail.double(), None, None, 1e-5, dt, tail.double())
+    close(y[-5:], *tols['y'], 'y')
+    assert not y[:-5].any()
+    dx, = torch.autograd.grad(y, x, x.detach())
+    h, tiny = half(dt)
+    ds, td = tols['ds']
+    close(dx[-5:], ds, td + h * (ds.abs() + td) + tiny, 'dx')
+    del x, y, dx
+    B, H, D = 1025, 128, 128                                              # a state of 2^31 elements and more
+    S = torch.zeros(B, 1, H, D, D, device='cuda')
+    c = decay_case(62, dt, 1, 1, 1, H, D, D)
+    S[-1] = c['state'][0].cuda()
+    q, k, v = (torch.zeros(B, 1, H, D, dtype=dt, device='cuda') for _ in range(3))
+    for a, n in ((q, 'q'), (k, 'k'), (v, 'v')):
+        a[-1] = c[n][0, 0].cuda()
+    ref, mag = decay_reference(c, D ** -0.5)
+    new = tp.decay_attention(q.unsqueeze(1), k.unsqueeze(1), v.unsqueeze(1), c['log_decay'].cuda(), state=S, return_state=True)[1]
+    close(new[-1:], ref['state'], decay_tol('state', ref, mag, c), 'new state')
+    o = tp.decay_attention_step(q, k, v, c['log_decay'].cuda(), S)
+    close(o[-1:].unsqueeze(1), ref['o'], decay_tol('o', ref, mag, c), 'o')
+    close(S[-1:], ref['state'], decay_tol('state', ref, mag, c), 'state')
+    assert not S[:-1].any() and not new[:-1].any()
+
+
+def test_second_derivatives_are_refused(tp):
+    t = together_inputs(torch.float32, 9)
+    calls = dict(rotary=lambda x: tp.rotary(x, t['pos'], t['f']), decay=lambda x: tp.decay_attention(x, t['k'], t['v'], t['ld']),
+                 norm=lambda x: tp.layer_norm(x, t['w'], t['b']), add=lambda x: tp.add_layer_norm(x, t['v'], t['w'], t['b'])[0])
+    for name, f in calls.items():
+        x = t['q'].detach().requires_grad_(True)
+        g, = torch.autograd.grad((f(x) ** 2).sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(g.sum(), x)
 
 
 def block_reference(mod, x, lengths):
