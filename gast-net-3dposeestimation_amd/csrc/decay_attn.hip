@@ -259,12 +259,19 @@ __device__ __forceinline__ void part_wild(const Frag<bf16_t>& f, Frag<bf16_t>& t
 struct View { const void* p; long t; int D; };           // token 0 of the sequence, its stride, channels
 template <typename T> struct Stage;
 template <> struct Stage<bf16_t> {
-    static constexpr int NV = 2;
+    static constexpr int NV = 2, VE = 8;
     uint4 x[NV];
     static __device__ __forceinline__ int row(int lane, int k) { return (lane >> 2) * 2 + k; }
     static __device__ __forceinline__ int chan(int wv, int lane, int) { return (wv * 4 + (lane & 3)) * 8; }
     __device__ __forceinline__ void none(int k) { x[k] = make_uint4(0, 0, 0, 0); }
-    __device__ __forceinline__ void vec(int k, const char* p) { x[k] = *(const uint4*)p; }
+    __device__ __forceinline__ void vec(int k, const char* p) { __builtin_memcpy(&x[k], p, 16); }
+    __device__ __forceinline__ void drop(int k, int n) {       // the first n elements
+        uint4 v = x[k];
+        if (n & 1) v = make_uint4(v.x >> 16 | v.y << 16, v.y >> 16 | v.z << 16, v.z >> 16 | v.w << 16, v.w >> 16);
+        if (n & 2) v = make_uint4(v.y, v.z, v.w, 0);
+        if (n & 4) v = make_uint4(v.z, v.w, 0, 0);
+        x[k] = v;
+    }
     __device__ __forceinline__ void some(int k, const bf16_t* p, int n) {
         uint32_t w[4] = {0, 0, 0, 0};
         for (int e = 0; e < 8 && e < n; ++e) w[e >> 1] |= (uint32_t)p[e] << 16 * (e & 1);
@@ -289,12 +296,18 @@ template <> struct Stage<bf16_t> {
     }
 };
 template <> struct Stage<float> {
-    static constexpr int NV = 4;
+    static constexpr int NV = 4, VE = 4;
     float4 x[NV];
     static __device__ __forceinline__ int row(int lane, int k) { return (lane >> 2) + 16 * (k >> 1); }
     static __device__ __forceinline__ int chan(int wv, int lane, int k) { return (wv * 8 + (lane & 3) + 4 * (k & 1)) * 4; }
     __device__ __forceinline__ void none(int k) { x[k] = make_float4(0.f, 0.f, 0.f, 0.f); }
-    __device__ __forceinline__ void vec(int k, const char* p) { x[k] = *(const float4*)p; }
+    __device__ __forceinline__ void vec(int k, const char* p) { __builtin_memcpy(&x[k], p, 16); }
+    __device__ __forceinline__ void drop(int k, int n) {
+        float4 v = x[k];
+        if (n & 1) v = make_float4(v.y, v.z, v.w, 0.f);
+        if (n & 2) v = make_float4(v.z, v.w, 0.f, 0.f);
+        x[k] = v;
+    }
     __device__ __forceinline__ void some(int k, const float* p, int n) {
         x[k] = make_float4(p[0], n > 1 ? p[1] : 0.f, n > 2 ? p[2] : 0.f, n > 3 ? p[3] : 0.f);
     }
@@ -311,24 +324,28 @@ template <> struct Stage<float> {
     }
 };
 // The loads of a chunk are issued while the one before is worked on, so they stand in straight code (a join of two paths would wait for
-// them): every lane reads a whole vector at a block-uniform base plus a 32-bit offset, at a row and channel that exist, and what is behind
-// the chunk's end or the head's last channel becomes zero on the way to LDS.
+// them): every lane reads 16 bytes at a block-uniform base plus a 32-bit offset, at a row and channels that exist (the last vector of a row
+// ends with the row), and what is behind the chunk's end or the head's last channel becomes zero on the way to LDS.  Rows may start
+// anywhere: this hardware's 16-byte accesses need no alignment of their own.
 template <typename T>
 __device__ __forceinline__ void bring(Stage<T>& s, const View& v, int t0, int n, int wv, int lane) {
     const char* base = (const char*)v.p + (long)t0 * v.t * (int)sizeof(T);
 #pragma unroll
     for (int k = 0; k < Stage<T>::NV; ++k) {
         const int d = Stage<T>::chan(wv, lane, k), row = min(Stage<T>::row(lane, k), n - 1);
-        s.vec(k, base + (uint32_t)(row * (int)v.t + (d < v.D ? d : 0)) * (uint32_t)sizeof(T));
+        s.vec(k, base + (uint32_t)(row * (int)v.t + min(d, v.D - Stage<T>::VE)) * (uint32_t)sizeof(T));
     }
 }
 template <typename T>
 __device__ __forceinline__ void trim(Stage<T>& s, const View& v, int n, int wv, int lane) {
 #pragma unroll
-    for (int k = 0; k < Stage<T>::NV; ++k)
-        if (Stage<T>::row(lane, k) >= n || Stage<T>::chan(wv, lane, k) >= v.D) s.none(k);
+    for (int k = 0; k < Stage<T>::NV; ++k) {
+        const int d = Stage<T>::chan(wv, lane, k);
+        if (v.D % Stage<T>::VE) s.drop(k, max(d + Stage<T>::VE - v.D, 0));
+        if (Stage<T>::row(lane, k) >= n || d >= v.D) s.none(k);
+    }
 }
-// rows that do not start on 16 bytes, or heads that do not end there: element by element, not ahead of time
+// heads shorter than a vector, tokens that lie too far apart: element by element, not ahead of time
 template <typename T>
 __device__ __forceinline__ void bring_odd(Stage<T>& s, const View& v, int t0, int n, int wv, int lane) {
 #pragma unroll
@@ -340,22 +357,23 @@ __device__ __forceinline__ void bring_odd(Stage<T>& s, const View& v, int t0, in
 }
 
 // Y (32 columns of out by 32 tokens, the token in lane % 32) to memory.  fp32: four registers are 16 bytes of a row, and go out as they are.
-__device__ __forceinline__ void put_tile(const f32x16& Y, float*, float* O, long st, int t0, int n, int c0, int D, int al, int lane) {
+__device__ __forceinline__ void put_tile(const f32x16& Y, float*, float* O, long st, int t0, int n, int c0, int D, int lane) {
     const int row = lane & 31;
     float* p = O + (long)(t0 + row) * st + c0 + 4 * (lane >> 5);
     const int left = D - c0 - 4 * (lane >> 5);
     if (row >= n) return;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-        if (al && 8 * q + 4 <= left) *(float4*)(p + 8 * q) = make_float4(Y[4 * q], Y[4 * q + 1], Y[4 * q + 2], Y[4 * q + 3]);
+        const float4 y = make_float4(Y[4 * q], Y[4 * q + 1], Y[4 * q + 2], Y[4 * q + 3]);
+        if (8 * q + 4 <= left) __builtin_memcpy(p + 8 * q, &y, 16);
         else
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
+            for (int e = 0; e < 3; ++e)
                 if (8 * q + e < left) p[8 * q + e] = Y[4 * q + e];
     }
 }
 // 16 bits: by way of LDS, so that a row leaves in 16-byte pieces
-__device__ __forceinline__ void put_tile(const f32x16& Y, bf16_t* tile, bf16_t* O, long st, int t0, int n, int c0, int D, int al, int lane) {
+__device__ __forceinline__ void put_tile(const f32x16& Y, bf16_t* tile, bf16_t* O, long st, int t0, int n, int c0, int D, int lane) {
 #pragma unroll
     for (int q = 0; q < 4; ++q)
         st4(tile + (lane & 31) * TS + 8 * q + 4 * (lane >> 5), make_float4(Y[4 * q], Y[4 * q + 1], Y[4 * q + 2], Y[4 * q + 3]));
@@ -368,9 +386,10 @@ __device__ __forceinline__ void put_tile(const f32x16& Y, bf16_t* tile, bf16_t* 
         if (row >= n || c0 + e >= D) continue;
         const bf16_t* s = tile + row * TS + e;
         bf16_t* p = O + (long)(t0 + row) * st + c0 + e;
-        if (al && c0 + e + 8 <= D) {
+        if (c0 + e + 8 <= D) {
             const uint2 u = *(const uint2*)s, w = *(const uint2*)(s + 4);
-            *(uint4*)p = make_uint4(u.x, u.y, w.x, w.y);
+            const uint4 y = make_uint4(u.x, u.y, w.x, w.y);
+            __builtin_memcpy(p, &y, 16);
         } else {
             for (int x = 0; x < 8 && c0 + e + x < D; ++x) p[x] = s[x];
         }
@@ -378,14 +397,14 @@ __device__ __forceinline__ void put_tile(const f32x16& Y, bf16_t* tile, bf16_t* 
 }
 // rows [t0, t1) of out are behind the sequence's end: zero (by nthr threads)
 template <typename T>
-__device__ __forceinline__ void put_zeros(T* O, long st, int t0, int t1, int D, int al, int tid, int nthr) {
+__device__ __forceinline__ void put_zeros(T* O, long st, int t0, int t1, int D, int tid, int nthr) {
     constexpr int VE = 16 / sizeof(T);
     const int nv = (D + VE - 1) / VE;
     for (long i = tid; i < (long)(t1 - t0) * nv; i += nthr) {
         const long t = i / nv;
         const int e = (int)(i - t * nv) * VE;
         T* p = O + (t0 + t) * st + e;
-        if (al && e + VE <= D) *(uint4*)p = make_uint4(0, 0, 0, 0);
+        if (e + VE <= D) __builtin_memset(p, 0, 16);
         else
             for (int x = 0; x < VE && e + x < D; ++x) p[x] = (T)0;
     }
@@ -402,13 +421,13 @@ struct Role {
     gast_seq out;
     const float* xin;                // X before the first token in this direction, [head][segment][D1][D2], or null: zero
     float* xout;                     // X behind the last, or null
-    int turn, reverse, D1, D2, al;   // turn: xin is held as [D2][D1]
+    int turn, reverse, D1, D2;       // turn: xin is held as [D2][D1]
     float fp, fk, fo;                // factors of scores, of what enters X, of what the carried X gives
 };
 
 struct ChunkArgs {
     gast_seq in[4];
-    int D[4], al[4];                 // channels; rows on 16 bytes
+    int D[4], vec[4];                // channels; can be read by vectors
     Role role[3];
     const float* log_decay;
     const int32_t* lengths;
@@ -451,6 +470,7 @@ __global__ void __launch_bounds__((Lay<DP, MODE>::NT), 2) chunk_kernel(const Chu
     using L = Lay<DP, MODE>;
     constexpr int NW = L::NW, RS = L::RS, G = DP / 32;
     constexpr bool BWD = MODE == TWO || MODE == THREE;
+    constexpr bool AHEAD = sizeof(T) == 2;
     extern __shared__ __align__(16) char lds[];
     using M = Lds<T, DP, MODE, STATE>;
     M& m = *(M*)lds;
@@ -565,8 +585,9 @@ __global__ void __launch_bounds__((Lay<DP, MODE>::NT), 2) chunk_kernel(const Chu
             Frag<T> fk[G];
             Exact<T> pv;
             auto enter = [&] {                             // c as it enters the state, and the other side of that product
+                if constexpr (AHEAD)
 #pragma unroll
-                for (int q = 0; q < G; ++q) fk[q] = ld_frag(tbT + 32 * q * TS, half);
+                    for (int q = 0; q < G; ++q) fk[q] = ld_frag(tbT + 32 * q * TS, half);
                 float v[16];
                 unpack(fc, v);
                 const float w = ro.fk * pw.per_unit[pa];
@@ -581,18 +602,18 @@ __global__ void __launch_bounds__((Lay<DP, MODE>::NT), 2) chunk_kernel(const Chu
                 if constexpr (STATE) px.set(X[0]);
 #pragma unroll
                 for (int q = 0; q < G; ++q) {
-                    if (q + 1 < G) na = ld_frag(ta + 32 * (q + 1), half), nb = ld_frag(tb + 32 * (q + 1), half);
+                    if (AHEAD && q + 1 < G) na = ld_frag(ta + 32 * (q + 1), half), nb = ld_frag(tb + 32 * (q + 1), half);
                     mma(P, fb, fa);
                     if constexpr (STATE) {
                         mma_fs(Y, px.v, fa);
                         if (q + 1 < G) nx.set(X[q + 1]);
-                        else enter();
+                        else if (AHEAD) enter();
                     }
+                    if (!AHEAD && q + 1 < G) na = ld_frag(ta + 32 * (q + 1), half), nb = ld_frag(tb + 32 * (q + 1), half);
                     fa = na; fb = nb; px = nx;
                 }
-            } else {
-                enter();
             }
+            if constexpr (MODE == SUMS || (STATE && !AHEAD)) enter();
             if constexpr (STATE)
                 if (renew) {
                     const float f = pw.unit[p] * pw.up[steps_on];
@@ -600,7 +621,10 @@ __global__ void __launch_bounds__((Lay<DP, MODE>::NT), 2) chunk_kernel(const Chu
                     for (int q = 0; q < G; ++q) X[q] *= f;
                 }
             // ---- X += b c; meanwhile the scores, and Y[e][i] += sum_j c_j[e] P[j][i]
-            if constexpr (STATE) mma_into<G>(X, fk, pv.v);
+            if constexpr (STATE && AHEAD) mma_into<G>(X, fk, pv.v);
+            if constexpr (STATE && !AHEAD)
+#pragma unroll
+                for (int q = 0; q < G; ++q) mma_sf(X[q], ld_frag(tbT + 32 * q * TS, half), pv.v);
             if constexpr (MODE != SUMS) {
                 float sc[16];
 #pragma unroll
@@ -633,7 +657,7 @@ __global__ void __launch_bounds__((Lay<DP, MODE>::NT), 2) chunk_kernel(const Chu
                 } else {
                     mma_sf(Y, fc, pp.v);
                 }
-                put_tile(Y, BWD ? m.tiles + NBUF * L::TILES + wave * 32 * TS : tc, O, ro.out.t, t0, n, wv * 32, D2, ro.al, lane);
+                put_tile(Y, BWD ? m.tiles + NBUF * L::TILES + wave * 32 * TS : tc, O, ro.out.t, t0, n, wv * 32, D2, lane);
             }
         }
         if constexpr (STATE) {
@@ -645,7 +669,7 @@ __global__ void __launch_bounds__((Lay<DP, MODE>::NT), 2) chunk_kernel(const Chu
             }
         }
     }
-    if (MODE != SUMS && s1 > max(e1, s0)) put_zeros<T>(O, ro.out.t, max(e1, s0), s1, D2, ro.al, tid - grp * NW * 64, NW * 64);
+    if (MODE != SUMS && s1 > max(e1, s0)) put_zeros<T>(O, ro.out.t, max(e1, s0), s1, D2, tid - grp * NW * 64, NW * 64);
     if (STATE && ro.xout && works) {
         float* xo = ro.xout + ((long)hd * g.nseg + seg) * (D1 * D2);
         const float f = pw.unit[p] * (MODE != SUMS && rev && len ? pw.up[1] : 1.f);
@@ -814,10 +838,10 @@ int launch_dp(const ChunkArgs& g, int dp, hipStream_t s) {
     if constexpr (MODE != THREE) return dp == 96 ? launch<T, 96, MODE, VEC, STATE>(g, s) : launch<T, 128, MODE, VEC, STATE>(g, s);
     return GAST_EINVAL;
 }
-// VEC: every tensor that is brought in has whole vectors.  STATE: there is a state to start from, to return or to hand to a second chunk.
+// VEC: every tensor that is brought in can be read by vectors.  STATE: there is a state to start from, to return or to hand to a second chunk.
 template <typename T, int MODE>
 int launch_any(const ChunkArgs& g, int dp, hipStream_t s) {
-    const bool vec = (MODE == SUMS || g.al[0]) && g.al[1] && g.al[2] && (MODE == ONE || MODE == SUMS || g.al[3]);
+    const bool vec = (MODE == SUMS || g.vec[0]) && g.vec[1] && g.vec[2] && (MODE == ONE || MODE == SUMS || g.vec[3]);
     if constexpr (MODE == ONE || MODE == THREE) {
         bool state = g.T > CT;
         for (const Role& r : g.role) state = state || r.xin || r.xout;
@@ -831,16 +855,15 @@ ChunkArgs chunk_args(const gast_decay_args& g, const Cut& c) {
     a.log_decay = g.log_decay; a.lengths = g.lengths; a.B = g.B; a.T = g.T; a.J = g.J; a.H = g.H; a.nseg = c.nseg; a.L = c.L;
     return a;
 }
-int on16(const gast_seq& s, int dtype) { return seq_align(s, dtype == GAST_F32 ? 4 : 2, dtype == GAST_F32 ? 4 : 8) == (dtype == GAST_F32 ? 4 : 8); }
 void put_in(ChunkArgs& a, int i, const gast_seq& s, int D, int dtype) {
     const int es = dtype == GAST_F32 ? 4 : 2;
     a.in[i] = s;
     a.D[i] = D;
-    a.al[i] = on16(s, dtype) && D % (16 / es) == 0 && s.t >= 0 && (CT * s.t + GAST_DECAY_MAX_D) * es < (1L << 31);      // (whole vectors, 32-bit offsets)
+    a.vec[i] = D >= 16 / es && s.t >= 0 && (CT * s.t + GAST_DECAY_MAX_D) * es < (1L << 31);      // (a vector fits, offsets fit 32 bits)
 }
-Role role_of(const gast_seq& out, int D1, int D2, int reverse, float scale, int dtype) {
+Role role_of(const gast_seq& out, int D1, int D2, int reverse, float scale) {
     Role r = {};
-    r.out = out; r.D1 = D1; r.D2 = D2; r.al = out.p ? on16(out, dtype) : 0; r.reverse = reverse;
+    r.out = out; r.D1 = D1; r.D2 = D2; r.reverse = reverse;
     r.fp = scale; r.fk = reverse ? scale : 1.f; r.fo = reverse ? 1.f : scale;
     return r;
 }
@@ -851,7 +874,7 @@ int states(const gast_decay_args& g, const Cut& c, const gast_seq& b, const gast
     ChunkArgs a = chunk_args(g, c);
     put_in(a, 1, b, g.Dk, g.dtype);
     put_in(a, 2, cc, g.Dv, g.dtype);
-    a.role[0] = role_of(gast_seq{}, g.Dk, g.Dv, reverse, g.scale, g.dtype);
+    a.role[0] = role_of(gast_seq{}, g.Dk, g.Dv, reverse, g.scale);
     a.role[0].xout = ws;
     a.skip_last = !last;
     if (int rc = launch_any<T, SUMS>(a, c.dp, s)) return rc;
@@ -868,7 +891,7 @@ int forward(const gast_decay_args& g, hipStream_t s) {
     put_in(a, 0, g.q, g.Dk, g.dtype);
     put_in(a, 1, g.k, g.Dk, g.dtype);
     put_in(a, 2, g.v, g.Dv, g.dtype);
-    a.role[0] = role_of(g.o, g.Dk, g.Dv, 0, g.scale, g.dtype);
+    a.role[0] = role_of(g.o, g.Dk, g.Dv, 0, g.scale);
     if (c.nseg > 1) {
         if (int rc = states<T>(g, c, g.k, g.v, 0, g.state, g.state_out, g.ws, s)) return rc;
         a.role[0].xin = g.ws;
@@ -898,13 +921,13 @@ int backward(const gast_decay_args& g, hipStream_t s) {
     put_in(a, 1, g.d_o, g.Dv, g.dtype);
     put_in(a, 2, g.k, g.Dk, g.dtype);
     put_in(a, 3, g.v, g.Dv, g.dtype);
-    a.role[0] = role_of(g.dv, g.Dk, g.Dv, 1, g.scale, g.dtype);
+    a.role[0] = role_of(g.dv, g.Dk, g.Dv, 1, g.scale);
     a.role[0].xin = behind;
     a.role[0].xout = c.nseg > 1 ? nullptr : g.dstate;
-    a.role[1] = role_of(g.dk, g.Dv, g.Dk, 1, g.scale, g.dtype);
+    a.role[1] = role_of(g.dk, g.Dv, g.Dk, 1, g.scale);
     a.role[1].xin = behind;
     a.role[1].turn = 1;
-    Role dq = role_of(g.dq, g.Dv, g.Dk, 0, g.scale, g.dtype);
+    Role dq = role_of(g.dq, g.Dv, g.Dk, 0, g.scale);
     dq.xin = before;
     dq.turn = 1;
     if (g.T <= CT && c.dp <= 64) {
