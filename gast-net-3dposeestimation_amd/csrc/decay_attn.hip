@@ -8,6 +8,7 @@
 // Forward in time the carry is decayed before it is used (o_t sees lambda S_(t-1)), backward in time the gradient of the last state is
 // used as it is and the decay follows: d state = lambda * (the recurrence's end).
 #include <atomic>
+#include <type_traits>
 #include "seq_common.h"
 
 namespace {
@@ -724,36 +725,37 @@ __global__ void __launch_bounds__(256) join_kernel(const JoinArgs g) {
     if (g.last) g.last[hd * g.size + i] = g.reverse && len ? power(lg, 1.f) * x : x;
 }
 
-// One token: a block per head, the state is read and written once (that is the whole cost: 8 Dk Dv bytes), VE columns a thread, the rows
-// spread over the other threads and summed through LDS.
-template <typename T, int VE>
+// One token: the state is read and written once (that is the whole cost: 8 Dk Dv bytes a head).  NT threads a head, VE columns a thread, the
+// rows spread over the other threads and summed through LDS.  Small states have heads of 64 threads, so that no thread is without work.
+template <typename T, int VE, int NT>
 __global__ void __launch_bounds__(256) step_kernel(const gast_decay_args p) {
-    __shared__ float sq[GAST_DECAY_MAX_D], sk[GAST_DECAY_MAX_D], so[256 * VE];
-    const int tid = threadIdx.x, Dk = p.Dk, Dv = p.Dv, nv = Dv / VE;
-    const long hd = blockIdx.x;
+    __shared__ float sq[256 / NT][GAST_DECAY_MAX_D], sk[256 / NT][GAST_DECAY_MAX_D], so[256 * VE];
+    const int tid = threadIdx.x % NT, grp = threadIdx.x / NT, Dk = p.Dk, Dv = p.Dv, nv = Dv / VE;
+    const long heads = (long)p.B * p.J * p.H, hd = min((long)blockIdx.x * (256 / NT) + grp, heads - 1);
+    const bool mine = (long)blockIdx.x * (256 / NT) + grp < heads;
     const int h = (int)(hd % p.H), j = (int)(hd / p.H % p.J);
     const long b = hd / p.H / p.J;
     T* O = (T*)p.o.p + seq_at(p.o, b, 0, j, h);
-    if (p.lengths && p.lengths[b] < 1) {
-        for (int e = tid; e < Dv; e += 256) Elem<T>::st(O + e, 0.f);
-        return;
-    }
+    const bool live = mine && !(p.lengths && p.lengths[b] < 1);
+    if (mine && !live)
+        for (int e = tid; e < Dv; e += NT) Elem<T>::st(O + e, 0.f);
     const T *Q = (const T*)p.q.p + seq_at(p.q, b, 0, j, h), *K = (const T*)p.k.p + seq_at(p.k, b, 0, j, h), *V = (const T*)p.v.p + seq_at(p.v, b, 0, j, h);
-    for (int d = tid; d < Dk; d += 256) {
-        sq[d] = Elem<T>::ld(Q + d) * p.scale;
-        sk[d] = Elem<T>::ld(K + d);
-    }
+    if (live)
+        for (int d = tid; d < Dk; d += NT) {
+            sq[grp][d] = Elem<T>::ld(Q + d) * p.scale;
+            sk[grp][d] = Elem<T>::ld(K + d);
+        }
     __syncthreads();
     // a lambda near 1 takes effect as lambda - 1: rounded itself, it would be off the same way at every token (10^4 tokens: 2^-11 of a state)
     const float lg = p.log_decay[h];
     const bool near = fabsf(lg) < 0.6931f;
     const float f = near ? expm1f(lg) : expf(lg);
-    const int rows = 256 / nv, c = tid % nv, r0 = tid / nv;
+    const int rows = NT / nv, c = tid % nv, r0 = tid / nv;
     float* S = (float*)p.state + hd * Dk * Dv + c * VE;
     float o[VE], v[VE];
 #pragma unroll
     for (int i = 0; i < VE; ++i) o[i] = 0.f;
-    if (r0 < rows) {
+    if (live && r0 < rows) {
 #pragma unroll
         for (int i = 0; i < VE; ++i) v[i] = Elem<T>::ld(V + c * VE + i);
 #pragma unroll 8
@@ -762,20 +764,21 @@ __global__ void __launch_bounds__(256) step_kernel(const gast_decay_args p) {
             ldv<VE>(x, S + d * Dv);
 #pragma unroll
             for (int i = 0; i < VE; ++i) {
-                x[i] = fmaf(f, x[i], fmaf(sk[d], v[i], near ? x[i] : 0.f));
-                o[i] = fmaf(sq[d], x[i], o[i]);
+                x[i] = fmaf(f, x[i], fmaf(sk[grp][d], v[i], near ? x[i] : 0.f));
+                o[i] = fmaf(sq[grp][d], x[i], o[i]);
             }
             stv<VE>(S + d * Dv, x);
         }
 #pragma unroll
-        for (int i = 0; i < VE; ++i) so[(r0 * nv + c) * VE + i] = o[i];
+        for (int i = 0; i < VE; ++i) so[grp * NT * VE + (r0 * nv + c) * VE + i] = o[i];
     }
     __syncthreads();
-    for (int e = tid; e < Dv; e += 256) {
-        float t = 0.f;
-        for (int r = 0; r < rows; ++r) t += so[r * Dv + e];
-        Elem<T>::st(O + e, t);
-    }
+    if (live)
+        for (int e = tid; e < Dv; e += NT) {
+            float t = 0.f;
+            for (int r = 0; r < rows; ++r) t += so[grp * NT * VE + r * Dv + e];
+            Elem<T>::st(O + e, t);
+        }
 }
 
 int check(const gast_decay_args* p) {
@@ -969,17 +972,26 @@ extern "C" int gast_decay_step(const gast_decay_args* args, gast_stream_t stream
     if (int rc = check(args)) return rc;
     if (!args->o.p || !args->state || args->T != 1) return GAST_EINVAL;
     const gast_decay_args& g = *args;
-    const long blocks = (long)g.B * g.J * g.H;
-    if (blocks > 0x7fffffffL) return GAST_ERANGE;
-    const int ve = ((uintptr_t)g.state % 16 == 0 && g.Dv % 4 == 0) ? 4 : 1;
+    const long heads = (long)g.B * g.J * g.H;
+    if (heads > 0x7fffffffL) return GAST_ERANGE;
     const hipStream_t s = (hipStream_t)stream;
-    const dim3 grid((unsigned)blocks), blk(256);
+    const int ve = (uintptr_t)g.state % 16 == 0 && g.Dv % 4 == 0 ? 4 : 1;
+    // 64 threads a head for states of up to 256 vectors (67456 heads of 16 x 16: 104 -> 42 us, 34816 of 32 x 32: 72 -> 57), 256 for larger ones
+    // (34816 of 31 x 64: 122 -> 109) and where there are too few heads to fill the card (17 of 32 x 32 either way 4 us of kernel)
+    const bool small = g.Dk * g.Dv <= ve * 256 && g.Dv <= 64 * ve && heads >= 1024;
+    const dim3 grid((unsigned)(small ? (heads + 3) / 4 : heads)), blk(256);
+    auto go = [&](auto t, auto v) {
+        using T = decltype(t);
+        constexpr int VE = decltype(v)::value;
+        if (small) hipLaunchKernelGGL((step_kernel<T, VE, 64>), grid, blk, 0, s, g);
+        else hipLaunchKernelGGL((step_kernel<T, VE, 256>), grid, blk, 0, s, g);
+    };
     if (g.dtype == GAST_F32) {
-        if (ve == 4) hipLaunchKernelGGL((step_kernel<float, 4>), grid, blk, 0, s, g);
-        else hipLaunchKernelGGL((step_kernel<float, 1>), grid, blk, 0, s, g);
+        if (ve == 4) go(float{}, std::integral_constant<int, 4>{});
+        else go(float{}, std::integral_constant<int, 1>{});
     } else {
-        if (ve == 4) hipLaunchKernelGGL((step_kernel<bf16_t, 4>), grid, blk, 0, s, g);
-        else hipLaunchKernelGGL((step_kernel<bf16_t, 1>), grid, blk, 0, s, g);
+        if (ve == 4) go(bf16_t{}, std::integral_constant<int, 4>{});
+        else go(bf16_t{}, std::integral_constant<int, 1>{});
     }
     GAST_CHECK_LAUNCH();
     return 0;
