@@ -185,12 +185,6 @@ __device__ __forceinline__ void mma_sf(f32x16& c, const Frag<bf16_t>& a, const P
 #endif
 }
 // X[q] += A[q] B for every q, one after the other: none waits for the one before
-template <int G> __device__ __forceinline__ void mma_into(f32x16 (&X)[G], const Frag<float> (&a)[G], const float (&b)[16]) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-#pragma unroll
-        for (int q = 0; q < G; ++q) X[q] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[q].x[i], b[i], X[q], 0, 0, 0);
-}
 template <int G> __device__ __forceinline__ void mma_into(f32x16 (&X)[G], const Frag<bf16_t> (&a)[G], const Parts& b) {
 #ifdef GAST_H16_F16
 #pragma unroll
@@ -471,6 +465,9 @@ __global__ void __launch_bounds__((Lay<DP, MODE>::NT), 2) chunk_kernel(const Chu
     using L = Lay<DP, MODE>;
     constexpr int NW = L::NW, RS = L::RS, G = DP / 32;
     constexpr bool BWD = MODE == TWO || MODE == THREE;
+    // 16 bits: operands are read and split a step ahead.  fp32: when they are needed -- its products are long and its operands take twice the
+    // registers (512 heads of 128 channels, 1024 tokens: 585 -> 489 us) -- and rows of X behind the last channel are left out (32 x 128 channels:
+    // 473 -> 249 us; at 16 bits the branches cost equal heads 2 to 3 % and gained unequal ones 4 to 17 %)
     constexpr bool AHEAD = sizeof(T) == 2;
     extern __shared__ __align__(16) char lds[];
     using M = Lds<T, DP, MODE, STATE>;
@@ -603,6 +600,7 @@ __global__ void __launch_bounds__((Lay<DP, MODE>::NT), 2) chunk_kernel(const Chu
                 if constexpr (STATE) px.set(X[0]);
 #pragma unroll
                 for (int q = 0; q < G; ++q) {
+                    if (!AHEAD && q && 32 * q >= D1) break;
                     if (AHEAD && q + 1 < G) na = ld_frag(ta + 32 * (q + 1), half), nb = ld_frag(tb + 32 * (q + 1), half);
                     mma(P, fb, fa);
                     if constexpr (STATE) {
@@ -622,10 +620,15 @@ __global__ void __launch_bounds__((Lay<DP, MODE>::NT), 2) chunk_kernel(const Chu
                     for (int q = 0; q < G; ++q) X[q] *= f;
                 }
             // ---- X += b c; meanwhile the scores, and Y[e][i] += sum_j c_j[e] P[j][i]
-            if constexpr (STATE && AHEAD) mma_into<G>(X, fk, pv.v);
-            if constexpr (STATE && !AHEAD)
+            if constexpr (STATE && AHEAD) {
+                mma_into<G>(X, fk, pv.v);
+            } else if constexpr (STATE) {
 #pragma unroll
-                for (int q = 0; q < G; ++q) mma_sf(X[q], ld_frag(tbT + 32 * q * TS, half), pv.v);
+                for (int q = 0; q < G; ++q) {
+                    if (q && 32 * q >= D1) break;
+                    mma_sf(X[q], ld_frag(tbT + 32 * q * TS, half), pv.v);
+                }
+            }
             if constexpr (MODE != SUMS) {
                 float sc[16];
 #pragma unroll
