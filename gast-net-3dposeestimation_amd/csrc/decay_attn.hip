@@ -911,15 +911,10 @@ int forward(const gast_decay_args& g, hipStream_t s) {
 template <typename T>
 int backward(const gast_decay_args& g, hipStream_t s) {
     const Cut c = cut(g.dtype, (long)g.B * g.J * g.H, g.T, g.Dk, g.Dv);
-    const long size = (long)g.B * g.J * g.H * c.nseg * g.Dk * g.Dv;
     const float *before = g.state, *behind = g.dstate_out;
     if (c.nseg > 1) {
-        before = g.ws_fwd;
-        if (!before) {
-            if (int rc = states<T>(g, c, g.k, g.v, 0, g.state, nullptr, g.ws + size, s)) return rc;
-            before = g.ws + size;
-        }
         if (int rc = states<T>(g, c, g.q, g.d_o, 1, g.dstate_out, g.dstate, g.ws, s)) return rc;
+        before = g.ws_fwd;
         behind = g.ws;
     }
     ChunkArgs a = chunk_args(g, c);
@@ -960,7 +955,7 @@ extern "C" int gast_decay_fwd(const gast_decay_args* args, gast_stream_t stream)
 extern "C" int gast_decay_bwd(const gast_decay_args* args, gast_stream_t stream) {
     if (int rc = check(args)) return rc;
     if (!args->d_o.p || !args->dq.p || !args->dk.p || !args->dv.p) return GAST_EINVAL;
-    if (!args->ws && gast_decay_ws_floats(args->dtype, args->B, args->T, args->J, args->H, args->Dk, args->Dv)) return GAST_EINVAL;
+    if ((!args->ws || !args->ws_fwd) && gast_decay_ws_floats(args->dtype, args->B, args->T, args->J, args->H, args->Dk, args->Dv)) return GAST_EINVAL;
     return args->dtype == GAST_F32 ? backward<float>(*args, (hipStream_t)stream) : backward<bf16_t>(*args, (hipStream_t)stream);
 }
 

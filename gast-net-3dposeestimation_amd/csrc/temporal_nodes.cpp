@@ -89,11 +89,14 @@ bool records(std::initializer_list<const Tensor*> ts) {
 Tensor or_none(const optional<Tensor>& t) { return t.has_value() ? *t : Tensor(); }
 optional<Tensor> maybe(const Tensor& t) { return t.defined() ? optional<Tensor>(t) : std::nullopt; }      // (nodes take no undefined inputs)
 
+constexpr int64_t MAX_AXIS = int64_t(1) << 30;         // (the C ABI counts in int)
+
 // (B, T, J, H, D) view of a (B, T, J, H, D) or (B, T, H, D) tensor, its channels contiguous
 Tensor heads(const char* what, const char* name, const Tensor& t) {
     const auto n = t.dim();
     TORCH_CHECK_VALUE(n == 4 || n == 5, what, ": ", name, " has to be (B, T, J, H, D) or (B, T, H, D), got ", t.sizes());
     for (int i = 2; i < n; ++i) TORCH_CHECK_VALUE(t.size(i) > 0, what, ": ", name, " has an empty axis: ", t.sizes());
+    for (int i = 0; i < n; ++i) TORCH_CHECK_VALUE(t.size(i) <= MAX_AXIS, what, ": ", name, " has an axis longer than ", MAX_AXIS, ": ", t.sizes());
     const Tensor c = t.stride(n - 1) == 1 || t.size(n - 1) == 1 ? t : t.contiguous();
     return n == 4 ? c.unsqueeze(2) : c;
 }
@@ -435,7 +438,7 @@ struct NormNode : torch::autograd::Function<NormNode> {
 variable_list norm(const std::string& what, const Tensor& x, const optional<Tensor>& residual_, const optional<Tensor>& weight_, const optional<Tensor>& bias_, double eps,
                    bool dropping, const optional<Tensor>& seed_, int64_t thresh, double inv_keep, int64_t salt) {
     const int64_t C = x.dim() ? x.size(-1) : 0;
-    TORCH_CHECK_VALUE(C > 0, what, ": x needs a last axis to normalise, got ", x.sizes());
+    TORCH_CHECK_VALUE(C > 0 && C <= MAX_AXIS, what, ": x needs a last axis of 1 to ", MAX_AXIS, " values to normalise, got ", x.sizes());
     const Tensor residual = or_none(residual_);
     Tensor weight = or_none(weight_), bias = or_none(bias_), seed = or_none(seed_);
     if (residual.defined())

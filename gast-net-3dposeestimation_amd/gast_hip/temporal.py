@@ -9,6 +9,11 @@ Tensors are (B, T, J, H, D) -- a sequence belongs to one joint of one clip, H he
 sequences; any strides, as long as a head's D values are contiguous (other tensors are copied first).  fp32, bfloat16 and float16; all of a
 call's activations have one type.  Everything is enqueued on the current stream of the tensors' device; there is no CPU fallback.  The
 checks, autograd nodes and kernel calls are csrc/temporal_nodes.cpp (gast_hip/_temporal.so).
+
+Every call can be captured into a HIP graph (workspaces come from torch's allocator, so every graph has its own), a backward pass together
+with its forward pass, on leaves made for the capture: no graph of the same leaves that was recorded outside the capture may be alive then,
+because autograd would make the capture wait for the stream of the older one.
+There is no second derivative: asking for one raises.
 """
 import os
 

@@ -527,7 +527,8 @@ long gast_layer_norm_bwd_ws_floats(long rows, int C);
 /* Causal linear attention with a decay for each head, lambda_h = exp(log_decay[h]):
  *   S_t = lambda S_(t-1) + k_t v_t',   o_t = scale q_t' S_t,   t < lengths[b] (null: T; clamped to 0 .. T)
  * S_(-1) = state ([B][J][H][Dk][Dv] fp32; null: zero), state_out (null: not wanted) = S behind the last token.  Outputs behind a
- * sequence's end are zero.  Dk, Dv <= GAST_DECAY_MAX_D. */
+ * sequence's end are zero.  Outputs overlap no input.  An infinity or NaN of a token reaches what sees the token and nothing else.
+ * Dk, Dv <= GAST_DECAY_MAX_D. */
 #define GAST_DECAY_MAX_D 128
 typedef struct {
     int dtype, B, T, J, H, Dk, Dv;
@@ -541,8 +542,8 @@ typedef struct {
     gast_seq d_o, dq, dk, dv;
     const float* dstate_out;
     float* dstate;
-    float* ws;                   /* gast_decay_ws_floats() floats (null where that is 0; backward without ws_fwd: twice as many) */
-    const float* ws_fwd;         /* backward: what gast_decay_fwd left in its ws for the same q, k, v, log_decay, lengths and state, or null */
+    float* ws;                   /* gast_decay_ws_floats() floats (null where that is 0) */
+    const float* ws_fwd;         /* backward: what gast_decay_fwd left in its ws for the same q, k, v, log_decay, lengths and state (null where ws may be) */
 } gast_decay_args;
 int gast_decay_fwd(const gast_decay_args* args, gast_stream_t stream);
 int gast_decay_bwd(const gast_decay_args* args, gast_stream_t stream);

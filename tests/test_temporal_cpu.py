@@ -1,9 +1,11 @@
 """gast_hip.temporal without a GPU: what the entry points refuse, the frequencies, and the 64-bit oracle against itself."""
+import ctypes
 import math
 
 import pytest
 import torch
 
+from gast_hip import binding
 from gast_hip import temporal as tp
 from gast_hip.binding import Dropout
 from oracle import temporal_oracle as to
@@ -123,3 +125,58 @@ def test_the_oracles_recurrence_is_the_sum_over_earlier_tokens():
     assert torch.allclose(o[:, :, 0], torch.einsum('bhts,bshe->bthe', a, v[:, :, 0]), rtol=1e-12, atol=1e-12)
     assert torch.allclose(S[:, 0], torch.einsum('bshd,hs,bshe->bhde', k[:, :, 0], torch.exp(ld[:, None] * (8 - t)), v[:, :, 0]), rtol=1e-12, atol=1e-12)
 
+
+
+def test_axes_that_an_int_cannot_count_are_refused():
+    """sizes reach the kernels as C ints: views of 2^32 + 5 tokens (of one stored token) must not come out as 5"""
+    T = 2 ** 32 + 5
+    x = z(1, 1, 1, 4).expand(1, T, 1, 4)
+    with pytest.raises(ValueError, match='longer than'):
+        tp.decay_attention(x, x, x, z(1))
+    with pytest.raises(ValueError, match='longer than'):
+        tp.rotary(x, torch.zeros(1, dtype=torch.int64).expand(T), tp.rotary_frequencies(4))
+    with pytest.raises(ValueError, match='longer than'):
+        tp.decay_attention_step(z(1, 1, 4).expand(T, 1, 4), z(1, 1, 4).expand(T, 1, 4), z(1, 1, 4).expand(T, 1, 4), z(1), z(1, 1, 1, 4, 4).expand(T, 1, 1, 4, 4))
+    with pytest.raises(ValueError, match='last axis'):
+        tp.layer_norm(z(1, 1).expand(1, T))
+
+
+class Seq(ctypes.Structure):
+    _fields_ = [('p', ctypes.c_void_p), ('b', ctypes.c_long), ('t', ctypes.c_long), ('j', ctypes.c_long), ('h', ctypes.c_long)]
+
+
+class DecayArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int) for n in ('dtype', 'B', 'T', 'J', 'H', 'Dk', 'Dv')] + [
+        ('scale', ctypes.c_float), ('log_decay', ctypes.c_void_p), ('lengths', ctypes.c_void_p)] + [(n, Seq) for n in ('q', 'k', 'v', 'o')] + [
+        ('state', ctypes.c_void_p), ('state_out', ctypes.c_void_p)] + [(n, Seq) for n in ('d_o', 'dq', 'dk', 'dv')] + [
+        (n, ctypes.c_void_p) for n in ('dstate_out', 'dstate', 'ws', 'ws_fwd')]
+
+
+def test_the_c_entries_refuse_what_is_missing():
+    """gast_decay_*: GAST_EINVAL (-1) or GAST_ERANGE before anything is launched"""
+    lib = ctypes.CDLL(binding.library_path(torch.bfloat16))
+    lib.gast_decay_ws_floats.restype = ctypes.c_long
+    some = ctypes.create_string_buffer(64)
+    at = ctypes.cast(some, ctypes.c_void_p).value
+
+    def args(**k):
+        a = DecayArgs(dtype=0, B=1, T=4096, J=1, H=1, Dk=32, Dv=32, scale=1.0, log_decay=at)
+        for n in ('q', 'k', 'v', 'o', 'd_o', 'dq', 'dk', 'dv'):
+            setattr(a, n, Seq(at, 0, 32, 0, 32))
+        a.ws = a.ws_fwd = at
+        for n, v in k.items():
+            setattr(a, n, v)
+        return a
+
+    assert lib.gast_decay_ws_floats(0, 1, 4096, 1, 1, 32, 32) > 0 and lib.gast_decay_ws_floats(0, 1, 32, 1, 1, 32, 32) == 0
+    assert lib.gast_decay_ws_floats(0, 0, 4096, 1, 1, 32, 32) == 0
+    for entry in ('fwd', 'bwd', 'step'):
+        call = getattr(lib, 'gast_decay_' + entry)
+        T = 1 if entry == 'step' else 4096
+        bad = [dict(B=0), dict(T=0), dict(J=-1), dict(H=0), dict(Dk=0), dict(Dv=0), dict(Dk=129), dict(Dv=129), dict(dtype=7), dict(log_decay=None), dict(q=Seq()),
+               dict(k=Seq()), dict(v=Seq()), dict(T=2 ** 30 + 1)]
+        bad += dict(fwd=[dict(o=Seq()), dict(ws=None)], bwd=[dict(d_o=Seq()), dict(dq=Seq()), dict(dk=Seq()), dict(dv=Seq()), dict(ws=None), dict(ws_fwd=None)],
+                    step=[dict(o=Seq()), dict(state=None), dict(state=at, T=2)])[entry]
+        for b in bad:
+            assert call(ctypes.byref(args(**dict(dict(T=T, state=at), **b))), None) < 0, (entry, b)
+        assert call(None, None) < 0
