@@ -21,12 +21,20 @@ namespace {
 // operands with the row (or column) in lane % 32 and any order of the summed index that both sides agree on.  Every operand here is held in
 // that same order -- 16 values a lane for 32 summed indexes -- so scores (summed over d, then over j) and states (made by a sum over j, then
 // summed over d) go from one product into the next without leaving their registers.  Only tokens pass through LDS, b and c turned on the way.
-// Scores are computed by every wave for itself: D / 16 of 11 D / 32 instructions at 128 channels, against a barrier and an LDS round trip.
+// Scores are computed by every wave for itself: at 128 channels 8 of a wave's 52 matrix instructions a chunk (16 bits), against a barrier and an
+// LDS round trip.
 //
 // Arithmetic.  fp32: fp32 matrix instructions.  16 bits: products of stored values are exact in fp32; scores and states, which are fp32,
 // meet 16-bit operands as two bf16 parts (hi = bf16(x), lo = bf16(x - hi): 2^-17 relative), what enters a state as three (all 24 bits: states
 // are results in fp32); in the binary16 flavour the stored operand is split into two bf16 parts as well (exactly; binary16 parts of a state
 // would overflow at 65504).  States are fp32 throughout.
+//
+// What bounds it, on a full card (two waves a SIMD, 1024 tokens, without gradients; a copy of the same bytes takes 112 us at 16 bits, 224 fp32):
+//   bf16  1024 heads of 64: 128 us, memory (4.2 TB/s); 512 of 128: 145 us, issue (586 vector, 52 matrix and 54 LDS instructions a wave and chunk:
+//         the splits into parts are most of them)
+//   fp16  64: 170 us, 128: 205 us: issue, both sides of a product are split
+//   fp32  2048 heads of 32: 327 us and 1024 of 64: 300 us, memory and LDS; 512 of 128: 490 - 540 us, of which 355 are matrix instructions
+// 16 heads of 128 channels and 32768 tokens (bf16) are cut into 32 segments: 80 us of sums, 14 of joining them, 175 of outputs.
 constexpr int CT = 32;               // tokens of a chunk
 constexpr int TS = CT + 4;           // row pitch of the turned tiles (elements): rows start 18 / 36 banks apart, no two of a read collide
 
@@ -728,20 +736,22 @@ __global__ void __launch_bounds__(256) join_kernel(const JoinArgs g) {
     if (g.last) g.last[hd * g.size + i] = g.reverse && len ? power(lg, 1.f) * x : x;
 }
 
-// One token: the state is read and written once (that is the whole cost: 8 Dk Dv bytes a head).  NT threads a head, VE columns a thread, the
+// One token: the state is read and written once (that is the whole cost: 8 Dk Dv bytes a head; 2048 heads of 128 x 128 in 57 us, 4.7 TB/s, the
+// rate of a copy).  NT threads a head, VE columns a thread, the
 // rows spread over the other threads and summed through LDS.  Small states have heads of 64 threads, so that no thread is without work.
 template <typename T, int VE, int NT>
 __global__ void __launch_bounds__(256) step_kernel(const gast_decay_args p) {
     __shared__ float sq[256 / NT][GAST_DECAY_MAX_D], sk[256 / NT][GAST_DECAY_MAX_D], so[256 * VE];
     const int tid = threadIdx.x % NT, grp = threadIdx.x / NT, Dk = p.Dk, Dv = p.Dv, nv = Dv / VE;
-    const long heads = (long)p.B * p.J * p.H, hd = min((long)blockIdx.x * (256 / NT) + grp, heads - 1);
-    const bool mine = (long)blockIdx.x * (256 / NT) + grp < heads;
+    const long heads = (long)p.B * p.J * p.H, hd = NT == 256 ? blockIdx.x : min((long)blockIdx.x * (256 / NT) + grp, heads - 1);
+    const bool mine = NT == 256 || (long)blockIdx.x * (256 / NT) + grp < heads;
     const int h = (int)(hd % p.H), j = (int)(hd / p.H % p.J);
     const long b = hd / p.H / p.J;
     T* O = (T*)p.o.p + seq_at(p.o, b, 0, j, h);
     const bool live = mine && !(p.lengths && p.lengths[b] < 1);
     if (mine && !live)
         for (int e = tid; e < Dv; e += NT) Elem<T>::st(O + e, 0.f);
+    if (NT == 256 && !live) return;
     const T *Q = (const T*)p.q.p + seq_at(p.q, b, 0, j, h), *K = (const T*)p.k.p + seq_at(p.k, b, 0, j, h), *V = (const T*)p.v.p + seq_at(p.v, b, 0, j, h);
     if (live)
         for (int d = tid; d < Dk; d += NT) {
