@@ -63,6 +63,14 @@ __device__ __forceinline__ Frag<bf16_t> ld_frag(const bf16_t* row, int half) {
     }
     return f;
 }
+// 16 values of a column: of a tile's rows (fp32, RS apart; p is the column's first value), or of a turned tile (16 bits; p is the column's row)
+template <int RS> __device__ __forceinline__ Frag<float> ld_column(const float* p, int half) {
+    Frag<float> f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) f.x[i] = p[(8 * (i >> 2) + 4 * half + (i & 3)) * RS];
+    return f;
+}
+template <int RS> __device__ __forceinline__ Frag<bf16_t> ld_column(const bf16_t* p, int half) { return ld_frag(p, half); }
 __device__ __forceinline__ void unpack(const Frag<float>& f, float (&v)[16]) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) v[i] = f.x[i];
@@ -219,42 +227,56 @@ template <> struct Prepared<bf16_t> { Split v; template <typename V> __device__ 
 template <typename T> struct Exact : Prepared<float> {};
 template <> struct Exact<bf16_t> { Parts v; __device__ __forceinline__ void set(const float (&x)[16]) { v = parts16(x); } };
 
-// Infinities and NaN among stored values: where they are zeros, and ones where they are (everything else zero)
+// Infinities and NaN among stored values: whether there are any; c += where they stand (ones) times which tokens are seen (sees(i): element i);
+// c += A B with zeros in their place.  These run for chunks that hold some; the fences keep their operands from being made all at once, for
+// the sake of the registers of everything else.
 __device__ __forceinline__ bool any_wild(const Frag<float>& f) {
     float t = 0.f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) t = fmaf(f.x[i], 0.f, t);
     return t != 0.f;
 }
-__device__ __forceinline__ void part_wild(const Frag<float>& f, Frag<float>& tame, Frag<float>& wild) {
+template <typename F> __device__ __forceinline__ void mma_wild(f32x16& c, const Frag<float>& f, const F& sees) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-        const bool w = !(fabsf(f.x[i]) < INFINITY);
-        tame.x[i] = w ? 0.f : f.x[i];
-        wild.x[i] = w ? 1.f : 0.f;
+        c = __builtin_amdgcn_mfma_f32_32x32x2f32(fabsf(f.x[i]) < INFINITY ? 0.f : 1.f, sees(i) ? 1.f : 0.f, c, 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+__device__ __forceinline__ void mma_tame(f32x16& c, const Frag<float>& f, const float (&b)[16]) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        c = __builtin_amdgcn_mfma_f32_32x32x2f32(fabsf(f.x[i]) < INFINITY ? f.x[i] : 0.f, b[i], c, 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
     }
 }
 // (16 bits: an exponent of all ones carries into the sign's place)
 #ifdef GAST_H16_F16
-constexpr uint32_t H_CARRY = 0x04000400u, H_ONE = 0x3c003c00u;
+constexpr uint32_t H_CARRY = 0x04000400u, H_ONE = 0x3c00u;
 #else
-constexpr uint32_t H_CARRY = 0x00800080u, H_ONE = 0x3f803f80u;
+constexpr uint32_t H_CARRY = 0x00800080u, H_ONE = 0x3f80u;
 #endif
 __device__ __forceinline__ uint32_t wild2(uint32_t x) { return ((x & 0x7fff7fffu) + H_CARRY) & 0x80008000u; }
 __device__ __forceinline__ bool any_wild(const Frag<bf16_t>& f) {
     return (wild2(f.x[0].x) | wild2(f.x[0].y) | wild2(f.x[0].z) | wild2(f.x[0].w) | wild2(f.x[1].x) | wild2(f.x[1].y) | wild2(f.x[1].z) | wild2(f.x[1].w)) != 0;
 }
-__device__ __forceinline__ void part_wild2(uint32_t x, uint32_t& tame, uint32_t& wild) {
-    const uint32_t w = (wild2(x) >> 15) * 0xffffu;
-    tame = x & ~w;
-    wild = H_ONE & w;
-}
-__device__ __forceinline__ void part_wild(const Frag<bf16_t>& f, Frag<bf16_t>& tame, Frag<bf16_t>& wild) {
+template <typename F> __device__ __forceinline__ void mma_wild(f32x16& c, const Frag<bf16_t>& f, const F& sees) {
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
-        part_wild2(f.x[q].x, tame.x[q].x, wild.x[q].x); part_wild2(f.x[q].y, tame.x[q].y, wild.x[q].y);
-        part_wild2(f.x[q].z, tame.x[q].z, wild.x[q].z); part_wild2(f.x[q].w, tame.x[q].w, wild.x[q].w);
+        auto one = [](uint32_t x) { return (wild2(x) >> 15) * H_ONE; };
+        auto see = [&](int i) { return (sees(i) ? H_ONE : 0u) | (sees(i + 1) ? H_ONE << 16 : 0u); };
+        c = mfma_h16(make_uint4(one(f.x[q].x), one(f.x[q].y), one(f.x[q].z), one(f.x[q].w)),
+                     make_uint4(see(8 * q), see(8 * q + 2), see(8 * q + 4), see(8 * q + 6)), c);
+        __builtin_amdgcn_sched_barrier(0);
     }
+}
+__device__ __forceinline__ void mma_tame(f32x16& c, const Frag<bf16_t>& f, const Split& b) {
+    auto tame = [](uint32_t x) { return x & ~((wild2(x) >> 15) * 0xffffu); };
+    Frag<bf16_t> t;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) t.x[q] = make_uint4(tame(f.x[q].x), tame(f.x[q].y), tame(f.x[q].z), tame(f.x[q].w));
+    mma_sf(c, t, b);
+    __builtin_amdgcn_sched_barrier(0);
 }
 
 // The 32 x DP tokens of one tensor on their way from memory to LDS: 16 elements a thread of NW waves.  16 bits: 8 channels of two rows,
@@ -317,13 +339,6 @@ template <> struct Stage<float> {
     template <int RS> __device__ __forceinline__ void rows(float* tile, int wv, int lane) const {
 #pragma unroll
         for (int k = 0; k < 4; ++k) *(float4*)(tile + row(lane, k) * RS + chan(wv, lane, k)) = x[k];
-    }
-    __device__ __forceinline__ void turned(float* tile, int wv, int lane) const {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            float* p = tile + chan(wv, lane, k) * TS + row(lane, k);
-            p[0] = x[k].x; p[TS] = x[k].y; p[2 * TS] = x[k].z; p[3 * TS] = x[k].w;
-        }
     }
 };
 // The loads of a chunk are issued while the one before is worked on, so they stand in straight code (a join of two paths would wait for
@@ -437,11 +452,14 @@ struct ChunkArgs {
     int B, T, J, H, nseg, L, skip_last;     // segments of L tokens; skip_last: nobody reads the sums of the last one in this direction
 };
 
-// LDS of a kernel, in elements: tiles as rows, turned tiles, output tiles of the waves (ONE: over the wave's own columns of c; fp32: none)
-template <int DP, int MODE> struct Lay {
-    static constexpr int NW = DP / 32, RS = DP + 4, ROWS = CT * RS, TURN = DP * TS;
+// LDS of a kernel, in elements: tiles as rows, turned tiles, output tiles of the waves (ONE: over the wave's own columns of c; fp32: none).
+// 16 bits need the turned tiles because an operand's register holds two tokens; fp32 reads columns of the rows, value by value, which takes LDS
+// as long as 16 bytes at a time, and has no room and no writes for them.
+template <typename T, int DP, int MODE> struct Lay {
+    static constexpr bool TURNED = sizeof(T) == 2;
+    static constexpr int NW = DP / 32, RS = DP + 4, ROWS = CT * RS, TURN = TURNED ? DP * TS : ROWS;
     static constexpr int GROUPS = MODE == TWO ? 2 : MODE == THREE ? 3 : 1, NT = GROUPS * NW * 64;
-    static constexpr int NROWS = MODE == ONE ? 2 : MODE == SUMS ? 0 : 4, NTURN = MODE == THREE ? 3 : 2;
+    static constexpr int NROWS = MODE == ONE ? (TURNED ? 2 : 3) : MODE == SUMS ? (TURNED ? 0 : 2) : 4, NTURN = !TURNED ? 0 : MODE == THREE ? 3 : 2;
     static constexpr int TILES = NROWS * ROWS + NTURN * TURN;
 };
 
@@ -459,7 +477,7 @@ struct Powers {
     float unit[PERIOD + 4], per_unit[PERIOD + 4];
 };
 template <typename T, int DP, int MODE, bool STATE> struct Lds {
-    using L = Lay<DP, MODE>;
+    using L = Lay<T, DP, MODE>;
     static constexpr int OUT = sizeof(T) == 2 && (MODE == TWO || MODE == THREE) ? L::NT / 64 * 32 * TS : 0;
     // two sets of tiles (one barrier a chunk instead of two) where the waves that the registers allow still fit: 20 KB a wave
     static constexpr int NBUF = STATE && (2 * L::TILES + OUT) * (int)sizeof(T) <= 20 * 1024 * L::GROUPS * L::NW ? 2 : 1;
@@ -467,10 +485,11 @@ template <typename T, int DP, int MODE, bool STATE> struct Lds {
     T tiles[NBUF * L::TILES + OUT];
 };
 
-
+// Two waves a SIMD where X lives in registers; four without a state (128 windows of 27 frames, 17 joints, 4 heads of 32 channels, fp32: the
+// backward pass takes 76 us with three, 72 with four, 93 with five, where registers spill).
 template <typename T, int DP, int MODE, bool VEC, bool STATE>
-__global__ void __launch_bounds__((Lay<DP, MODE>::NT), 2) chunk_kernel(const ChunkArgs g) {
-    using L = Lay<DP, MODE>;
+__global__ void __launch_bounds__((Lay<T, DP, MODE>::NT), (STATE ? 2 : 4)) chunk_kernel(const ChunkArgs g) {
+    using L = Lay<T, DP, MODE>;
     constexpr int NW = L::NW, RS = L::RS, G = DP / 32;
     constexpr bool BWD = MODE == TWO || MODE == THREE;
     // 16 bits: operands are read and split a step ahead.  fp32: when they are needed -- its products are long and its operands take twice the
@@ -494,8 +513,10 @@ __global__ void __launch_bounds__((Lay<DP, MODE>::NT), 2) chunk_kernel(const Chu
     const float lg = g.log_decay[h];
     // ---- roles: dv (a, b, c) = (k, q, do), dk (v, do, q), dq (do, v, k); turned tiles of BWD: q, do (, k)
     const int ia = BWD ? (grp == 0 ? 2 : grp == 1 ? 3 : 1) : 0, ib = BWD ? (grp == 0 ? 0 : grp == 1 ? 1 : 3) : 1, ic = BWD ? (grp == 0 ? 1 : grp == 1 ? 0 : 2) : 2;
-    const int oa = ia * L::ROWS, ob = ib * L::ROWS, obT = TURN0 + (BWD ? ib : 0) * L::TURN;       // offsets in a set of tiles
-    const int oc = TURN0 + (BWD ? ic : 1) * L::TURN + wv * 32 * TS;                               // (this wave's 32 columns of c)
+    // offsets in a set of tiles: rows, and columns of turned tiles or of rows
+    constexpr int COL0 = L::TURNED ? TURN0 : MODE == ONE ? L::ROWS : 0, CS = L::TURNED ? TS : 1;       // (the columns of b of ONE and SUMS; a column's step)
+    const int oa = ia * L::ROWS, ob = ib * L::ROWS, obT = COL0 + (BWD ? ib : 0) * L::TURN;
+    const int oc = COL0 + (BWD ? ic : 1) * L::TURN + wv * 32 * CS;                                // (this wave's 32 columns of c)
     const int c0 = wv * 32 + col, D1 = ro.D1, D2 = ro.D2;
     const bool works = wv * 32 < D2;
 
@@ -524,8 +545,9 @@ __global__ void __launch_bounds__((Lay<DP, MODE>::NT), 2) chunk_kernel(const Chu
             if (st[i] < 0) continue;
             if constexpr (VEC) { if (!whole || n < CT) trim<T>(stage[i], in[i], n, wv, lane); }
             else bring_odd<T>(stage[i], in[i], t0, n, wv, lane);
-            if (MODE == ONE ? i < 2 : MODE != SUMS) stage[i].template rows<RS>(tiles + st[i] * L::ROWS, wv, lane);
-            if (MODE == ONE ? i > 0 : MODE == SUMS || st[i] < L::NTURN) stage[i].turned(tiles + TURN0 + (BWD ? st[i] : st[i] - 1) * L::TURN, wv, lane);
+            if (!L::TURNED || (MODE == ONE ? i < 2 : MODE != SUMS)) stage[i].template rows<RS>(tiles + (MODE == SUMS ? i : st[i]) * L::ROWS, wv, lane);
+            if constexpr (L::TURNED)
+                if (MODE == ONE ? i > 0 : MODE == SUMS || st[i] < L::NTURN) stage[i].turned(tiles + TURN0 + (BWD ? st[i] : st[i] - 1) * L::TURN, wv, lane);
         }
     };
     const int c_first = rev && MODE != THREE ? nchunk - 1 : 0;
@@ -583,17 +605,17 @@ __global__ void __launch_bounds__((Lay<DP, MODE>::NT), 2) chunk_kernel(const Chu
         const int pa = renew ? 0 : p + 1;                   // the unit afterwards
         if constexpr (STATE) fetch(next);                  // (the last chunk once more: no branch here)
         if (works) {
-            const T *ta = tiles + oa + col * RS, *tb = tiles + ob + col * RS, *tbT = tiles + obT + col * TS;
+            const T *ta = tiles + oa + col * RS, *tb = tiles + ob + col * RS, *tbT = tiles + obT + col * CS;
             T* const tc = tiles + oc;
             // ---- P[j][i] = b_j a_i, Y[e][i] = sum_d X[d][e] a_i[d].  What one step's products need is read and split during the step before.
             f32x16 P = {}, Y = {};
-            const Frag<T> fc = ld_frag(tc + col * TS, half);
+            const Frag<T> fc = ld_column<RS>(tc + col * CS, half);
             Frag<T> fk[G];
             Exact<T> pv;
             auto enter = [&] {                             // c as it enters the state, and the other side of that product
                 if constexpr (AHEAD)
 #pragma unroll
-                    for (int q = 0; q < G; ++q) fk[q] = ld_frag(tbT + 32 * q * TS, half);
+                    for (int q = 0; q < G; ++q) fk[q] = ld_column<RS>(tbT + 32 * q * CS, half);
                 float v[16];
                 unpack(fc, v);
                 const float w = ro.fk * pw.per_unit[pa];
@@ -634,7 +656,7 @@ __global__ void __launch_bounds__((Lay<DP, MODE>::NT), 2) chunk_kernel(const Chu
 #pragma unroll
                 for (int q = 0; q < G; ++q) {
                     if (q && 32 * q >= D1) break;
-                    mma_sf(X[q], ld_frag(tbT + 32 * q * TS, half), pv.v);
+                    mma_sf(X[q], ld_column<RS>(tbT + 32 * q * CS, half), pv.v);
                 }
             }
             if constexpr (MODE != SUMS) {
@@ -650,19 +672,13 @@ __global__ void __launch_bounds__((Lay<DP, MODE>::NT), 2) chunk_kernel(const Chu
                 if constexpr (STATE) wild = !(fabsf(X[0][0]) < INFINITY);
                 else wild = any_wild(fc);
                 if (__any(wild)) {
-                    Frag<T> tame, ones;
-                    part_wild(fc, tame, ones);
                     f32x16 Z = {};
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) sc[r] = (8 * (r >> 2) + 4 * half + (r & 3) - col) * (rev ? 1 : -1) >= 0 ? 1.f : 0.f;
-                    Prepared<T> sees;
-                    sees.set(sc);
-                    mma_sf(Z, ones, sees.v);
+                    mma_wild(Z, fc, [&](int r) { return (8 * (r >> 2) + 4 * half + (r & 3) - col) * (rev ? 1 : -1) >= 0; });
                     uint32_t at = 0;
 #pragma unroll
                     for (int r = 0; r < 16; ++r) at |= Z[r] != 0.f ? 1u << r : 0u;
                     Z = Y;
-                    mma_sf(Z, tame, pp.v);
+                    mma_tame(Z, fc, pp.v);
                     mma_sf(Y, fc, pp.v);
 #pragma unroll
                     for (int r = 0; r < 16; ++r) Y[r] = at >> r & 1 ? Y[r] : Z[r];
@@ -829,7 +845,7 @@ Cut cut(int dtype, long heads, int T, int Dk, int Dv) {
 
 template <typename T, int DP, int MODE, bool VEC, bool STATE>
 int launch(const ChunkArgs& g, hipStream_t s) {
-    using L = Lay<DP, MODE>;
+    using L = Lay<T, DP, MODE>;
     constexpr int bytes = (int)sizeof(Lds<T, DP, MODE, STATE>);
     const long blocks = (long)g.B * g.J * g.H * g.nseg;
     if (blocks > 0x7fffffffL) return GAST_ERANGE;
