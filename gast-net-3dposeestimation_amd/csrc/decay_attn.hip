@@ -7,6 +7,7 @@
 //   dv  a = k,  b = q,  c = do   backward in time           dk  a = v,  b = do, c = q    backward in time (X = the transposed one of dv)
 // Forward in time the carry is decayed before it is used (o_t sees lambda S_(t-1)), backward in time the gradient of the last state is
 // used as it is and the decay follows: d state = lambda * (the recurrence's end).
+#include <algorithm>
 #include <atomic>
 #include <type_traits>
 #include "seq_common.h"
@@ -820,19 +821,26 @@ int check(const gast_decay_args* p) {
 
 // How the tokens are cut into segments, each with blocks of its own that start from the state before it.  In units of one chunk's work of a
 // block: a cut reads two of the tensors twice (half a chunk's work for each chunk), hands a state of D x D fp32 over four times for each segment
-// (as many bytes as D / 16 chunks of 16-bit tokens have, D / 32 of fp32), and has two launches more (about 6); blocks that run at once are two
-// waves to each of the 1024 SIMDs.  Measured: 16 heads of 128 channels and 32768 tokens (bf16, forward) take 2336 us uncut, 277 in 32 segments.
+// (as many bytes as D / 16 chunks of 16-bit tokens have, D / 32 of fp32), and has two launches more (about 6 chunks' time, 4 of the longer fp32
+// ones).  A CU runs eight waves' worth of blocks at once, two to a SIMD; a last round that is not full still takes half of one.
+// Measured, uncut and cut: 16 heads of 128 channels and 32768 tokens (bf16, forward) 1937 us in two segments, 272 in 32; forward and backward in fp32,
+// 12 heads of 16 and 530 tokens 203 and 44 in 17, 128 heads of 64 and 362 tokens 189 and 140 in 6.
 struct Cut { int dp, nseg, L; };
 Cut cut(int dtype, long heads, int T, int Dk, int Dv) {
     const int D = Dk > Dv ? Dk : Dv;
     Cut c;
     c.dp = (D + 31) / 32 * 32;
-    const long slots = 2048 * 32 / c.dp, chunks = (T + CT - 1L) / CT;
-    const double state = 2 + c.dp / (dtype == GAST_F32 ? 32.0 : 16.0);
-    double best = (double)((heads + slots - 1) / slots) * chunks;
+    const long slots = 256 * (8 * 32 / c.dp), chunks = (T + CT - 1L) / CT;
+    const double state = 2 + c.dp / (dtype == GAST_F32 ? 32.0 : 16.0), launches = dtype == GAST_F32 ? 4 : 6;
+    auto rounds = [&](long blocks) {
+        const long full = blocks / slots, rest = blocks % slots;
+        return !rest ? (double)full : !full ? 1.0 : full + std::max(0.5, (double)rest / slots);
+    };
+    double best = (double)chunks;
     long nseg = 1;
-    for (long n = 2; n <= 64 && n * 2 <= chunks && heads < slots; ++n) {
-        const double t = (double)((heads * n + slots - 1) / slots) * (1.5 * ((chunks + n - 1) / n) + state) + 6;
+    for (long n = 2; n <= 64 && n <= chunks && heads < slots; ++n) {
+        const long len = (chunks + n - 1) / n;
+        const double t = rounds(heads * ((chunks + len - 1) / len)) * (1.5 * len + state) + launches;
         if (t < best) {
             best = t;
             nseg = n;

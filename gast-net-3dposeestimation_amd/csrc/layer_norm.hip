@@ -11,7 +11,7 @@
 // registers over all its rows, groups of a block meet in LDS, blocks in a partial row each, and a second launch adds the partial rows in a
 // fixed order (no atomics: run-to-run the same bits).
 // Measured: 8192 rows of 4096 (bf16, dropout) 53 us forward = 5.0 TB/s, 76 + 6 us backward = 4.4 TB/s (a copy reaches 4.8); 58752 rows of 128
-// (fp32) 14 + 20 us.
+// (fp32) 12 us forward, 16 + 4 us backward.
 #include "seq_common.h"
 
 namespace {

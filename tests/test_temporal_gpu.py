@@ -112,6 +112,31 @@ def test_rotary_copies_what_is_not_turned_and_keeps_empty_calls(tp):
     assert e.shape == (0, 2, 1, 2, 8)
 
 
+def test_rotary_in_place_through_the_c_abi(tp):
+    """y may be x: the vector at a row's end overlaps the one before it, which another thread may have turned already"""
+    import ctypes
+
+    from gast_hip import binding
+
+    class Seq(ctypes.Structure):
+        _fields_ = [('p', ctypes.c_void_p)] + [(n, ctypes.c_long) for n in 'btjh']
+
+    class Job(ctypes.Structure):
+        _fields_ = [('x', Seq), ('y', Seq), ('H', ctypes.c_int)]
+
+    B, T, J, H = 2, 300, 1, 3
+    for dt in (torch.float32, torch.bfloat16):
+        lib = ctypes.CDLL(binding.library_path(dt))
+        for D, R, inter in ((18, 18, 0), (18, 18, 1), (45, 22, 0), (45, 22, 1), (128, 64, 0)):
+            x, f, pos = randn(gen(D), dt, B, T, J, H, D).cuda(), tp.rotary_frequencies(R).cuda(), torch.arange(T).cuda()
+            want = tp.rotary(x, pos, f, interleaved=bool(inter))
+            job = Job(*[Seq(x.data_ptr(), *x.stride()[:4])] * 2, H)
+            rc = lib.gast_rotary_multi(0 if dt == torch.float32 else 1, ctypes.byref(job), 1, B, T, J, D, R, inter, ctypes.c_void_p(pos.data_ptr()), 1,
+                                       ctypes.c_long(0), ctypes.c_long(1), ctypes.c_void_p(f.data_ptr()), ctypes.c_float(1.0), 0,
+                                       ctypes.c_void_p(torch.cuda.current_stream().cuda_stream))
+            assert rc == 0 and torch.equal(x, want), (dt, D, R, inter)
+
+
 # ------------------------------------------------------------------------------------------------ linear attention with a decay
 def decay_case(seed, dt, B, T, J, H, Dk, Dv, ragged=False, state=True, decays=None):
     g = gen(seed)
