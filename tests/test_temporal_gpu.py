@@ -255,6 +255,13 @@ def test_decay_long(tp, dt):
     check_decay(tp, decay_case(8, dt, 2, 1500, 1, 1, 64, 64, ragged=True, decays=[-0.001]))
 
 
+@pytest.mark.parametrize('dt', TYPES, ids=IDS)
+@pytest.mark.parametrize('B,T,H,Dk,Dv', [(1, 530, 3, 16, 16), (3, 362, 4, 64, 48), (2, 700, 2, 128, 96), (2, 300, 2, 31, 87), (3, 65, 1, 128, 8), (1, 2050, 1, 7, 128)])
+def test_decay_segments(tp, dt, B, T, H, Dk, Dv):
+    """a few chunks a segment down to one, clips that end before a segment begins, states at both ends"""
+    check_decay(tp, decay_case(B + T, dt, B, T, 1, H, Dk, Dv, ragged=B > 1, decays=[-0.01, -0.0005, -2.0, 0.0]))
+
+
 WILD = [(20, 32, [(7, 'nan'), (19, 'inf')]), (27, 64, [(13, '-inf')]), (32, 96, [(0, 'inf'), (31, 'nan')]), (200, 48, [(40, 'inf'), (170, 'nan')]), (130, 128, [(96, 'nan')]),
         (3000, 64, [(1500, 'nan')])]
 
