@@ -183,29 +183,21 @@ template <typename V> __device__ __forceinline__ Parts parts16(const V& v) {
         }
     return s;
 }
-__device__ __forceinline__ void mma_sf(f32x16& c, const Frag<bf16_t>& a, const Parts& b) {
-#ifdef GAST_H16_F16
-    const Split p = stored_parts(a);
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-        c = mfma_pair<1>(p.hi[q], b.x[2][q], c);
-        c = mfma_pair<1>(p.lo[q], b.x[1][q], c);
-        c = mfma_pair<1>(p.hi[q], b.x[1][q], c);
-        c = mfma_pair<1>(p.lo[q], b.x[0][q], c);
-        c = mfma_pair<1>(p.hi[q], b.x[0][q], c);
-    }
-#else
-#pragma unroll
-    for (int q = 0; q < 2; ++q)
-#pragma unroll
-        for (int k = 2; k >= 0; --k) c = mfma_pair<1>(a.x[q], b.x[k][q], c);
-#endif
-}
-// X[q] += A[q] B for every q, one after the other: none waits for the one before
+// X[q] += A[q] B for every q (bf16: one after the other, so that none waits for the one before)
 template <int G> __device__ __forceinline__ void mma_into(f32x16 (&X)[G], const Frag<bf16_t> (&a)[G], const Parts& b) {
 #ifdef GAST_H16_F16
 #pragma unroll
-    for (int q = 0; q < G; ++q) mma_sf(X[q], a[q], b);
+    for (int q = 0; q < G; ++q) {
+        const Split p = stored_parts(a[q]);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            X[q] = mfma_pair<1>(p.hi[s], b.x[2][s], X[q]);
+            X[q] = mfma_pair<1>(p.lo[s], b.x[1][s], X[q]);
+            X[q] = mfma_pair<1>(p.hi[s], b.x[1][s], X[q]);
+            X[q] = mfma_pair<1>(p.lo[s], b.x[0][s], X[q]);
+            X[q] = mfma_pair<1>(p.hi[s], b.x[0][s], X[q]);
+        }
+    }
 #else
 #pragma unroll
     for (int k = 2; k >= 0; --k)
