@@ -404,6 +404,8 @@ struct NormNode : torch::autograd::Function<NormNode> {
         return r.stream.defined() ? variable_list{r.y, r.stream} : variable_list{r.y};
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        // (a node is called with no gradient at all where the one behind it gave none)
+        if (!grads[0].defined() && (grads.size() < 2 || !grads[1].defined())) return variable_list(9);
         const auto s = ctx->get_saved_variables();
         const Tensor S = rows_of(s[0]), &weight = s[1], &stats = s[2], &seed = s[3];
         const int64_t rows = S.size(0), C = S.size(1);

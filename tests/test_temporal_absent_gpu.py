@@ -1,0 +1,61 @@
+"""Gradients that are not there: a node of gast_hip.temporal whose outputs nobody differentiates is called without one."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope='module')
+def tp():
+    from gast_hip import temporal
+    return temporal
+
+
+class Mute(torch.autograd.Function):
+    """passes its inputs on and has no gradient for them"""
+
+    @staticmethod
+    def forward(ctx, *xs):
+        return sum(x.float().sum() for x in xs)
+
+    @staticmethod
+    def backward(ctx, d):
+        return (None,) * len(ctx.needs_input_grad)
+
+
+def leaf(*shape):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(sum(shape))).cuda().requires_grad_(True)
+
+
+def nothing(out, leaves):
+    got = torch.autograd.grad(Mute.apply(*out), leaves, allow_unused=True)
+    assert all(g is None or not g.any() for g in got), got
+
+
+def test_layer_norm_without_a_gradient(tp):
+    x, w, b = leaf(5, 32), leaf(32), leaf(32)
+    nothing((tp.layer_norm(x, w, b),), [x, w, b])
+    nothing((tp.layer_norm(x),), [x])
+
+
+@pytest.mark.parametrize('p', [0.0, 0.5])
+def test_add_layer_norm_without_a_gradient(tp, p):
+    from gast_hip.binding import Dropout, dropout_params
+    drop = Dropout(torch.tensor([3], dtype=torch.int32).cuda(), *dropout_params(p)) if p else None
+    x, r, w, b = leaf(5, 3, 32), leaf(5, 3, 32), leaf(32), leaf(32)
+    y, s = tp.add_layer_norm(x, r, w, b, drop=drop)
+    nothing((y, s), [x, r, w, b])
+    # one of the outputs alone: the other's gradient counts
+    y, s = tp.add_layer_norm(x, r, w, b, drop=drop)
+    got = torch.autograd.grad(Mute.apply(y) + s.sum(), [x, r, w, b], allow_unused=True)
+    assert torch.equal(got[1], torch.ones_like(r)) and not got[2].any() and not got[3].any()
+
+
+def test_the_other_operators_without_a_gradient(tp):
+    q, k, v, s = leaf(2, 40, 1, 2, 8), leaf(2, 40, 1, 2, 8), leaf(2, 40, 1, 2, 16), leaf(2, 1, 2, 8, 16)
+    ld = torch.full((2,), -0.1, device='cuda')
+    nothing((tp.decay_attention(q, k, v, ld),), [q, k, v])
+    nothing(tp.decay_attention(q, k, v, ld, state=s, return_state=True), [q, k, v, s])
+    f = tp.rotary_frequencies(8).cuda()
+    nothing((tp.rotary(q, torch.arange(40).cuda(), f),), [q])
+    nothing(tp.rotary((q, k), torch.arange(40).cuda(), f), [q, k])
