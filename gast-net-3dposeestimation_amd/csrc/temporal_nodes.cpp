@@ -110,14 +110,15 @@ Tensor last_contiguous(const Tensor& t) { return t.stride(-1) == 1 || t.size(-1)
 Tensor floats(const Tensor& like, at::IntArrayRef shape) { return at::empty(shape, like.options().dtype(at::kFloat)); }
 Tensor fresh(const Tensor& like) { return at::empty(like.sizes(), like.options()); }
 
-// there is no second derivative: a gradient that is itself recorded gets a node that says so
-variable_list first_order(const char* what, const variable_list& grads, variable_list outs) {
+// There is no second derivative: a gradient that is recorded, or that is made from an input of the call that is (of[i], for outs[i]), gets a
+// node that says so.
+variable_list first_order(const char* what, const variable_list& grads, variable_list outs, std::initializer_list<bool> of = {}) {
     if (!at::GradMode::is_enabled()) return outs;
     bool any = false;
     for (const Tensor& g : grads) any = any || (g.defined() && g.requires_grad());
-    if (!any) return outs;
-    for (Tensor& o : outs) {
-        if (!o.defined()) continue;
+    for (size_t i = 0; i < outs.size(); ++i) {
+        Tensor& o = outs[i];
+        if (!o.defined() || !(any || (i < of.size() && of.begin()[i]))) continue;
         Tensor d = o.detach();
         d.set_requires_grad(true);
         o = (*std::make_shared<torch::autograd::DelayedError>(std::string(what) + ": trying to differentiate twice, there is no second derivative", 1))({d})[0];
@@ -259,6 +260,7 @@ struct DecayNode : torch::autograd::Function<DecayNode> {
         variable_list out = decay_forward(q, k, v, log_decay, state, lengths, scale, want_state, &segments);
         ctx->save_for_backward({q, k, v, log_decay, state, lengths, segments});
         ctx->saved_data["scale"] = scale;
+        ctx->saved_data["trained"] = (int64_t)(q.requires_grad() + 2 * k.requires_grad() + 4 * v.requires_grad() + 8 * (state.defined() && state.requires_grad()));
         ctx->set_materialize_grads(false);
         return out;
     }
@@ -284,7 +286,10 @@ struct DecayNode : torch::autograd::Function<DecayNode> {
             if (dnext.defined()) dstate.copy_(dnext);
             else dstate.zero_();
         }
-        return first_order("decay_attention", grads, {dq, dk, dv, Tensor(), dstate, Tensor(), Tensor(), Tensor()});
+        // (the outputs are linear in each input: a gradient is made from the others)
+        const int64_t t = ctx->saved_data["trained"].toInt();
+        const bool tq = t & 1, tk = t & 2, tv = t & 4, ts = t & 8;
+        return first_order("decay_attention", grads, {dq, dk, dv, Tensor(), dstate, Tensor(), Tensor(), Tensor()}, {tk || tv || ts, tq || tv, tq || tk, false, tq});
     }
 };
 
@@ -395,6 +400,8 @@ struct NormNode : torch::autograd::Function<NormNode> {
                                  const optional<Tensor>& bias_, const optional<Tensor>& seed_, double eps, int64_t thresh, double inv_keep, int64_t salt) {
         const Tensor residual = or_none(residual_), weight = or_none(weight_), bias = or_none(bias_), seed = or_none(seed_);
         ctx->saved_data["given"] = (int64_t)(residual.defined() + 2 * weight.defined() + 4 * bias.defined());
+        const bool stream = x.requires_grad() || (residual.defined() && residual.requires_grad());
+        ctx->saved_data["trained"] = (int64_t)(stream + 2 * (weight.defined() && weight.requires_grad()));
         const NormOut r = norm_forward(x, residual, weight, bias, seed, eps, {thresh, inv_keep, salt}, true);
         ctx->save_for_backward({r.stream.defined() ? r.stream : r.normed, weight, r.stats, seed});
         ctx->saved_data["thresh"] = thresh;
@@ -433,7 +440,10 @@ struct NormNode : torch::autograd::Function<NormNode> {
             if (want_w) dw.zero_();
             if (want_b) db.zero_();
         }
-        return first_order("layer_norm", grads, {want_x ? (shared ? dS : dX) : Tensor(), want_r ? dS : Tensor(), dw, db, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()});
+        // (the stream's gradient is made from the stream and the weight, the weight's from the stream, the bias' from neither)
+        const int64_t t = ctx->saved_data["trained"].toInt();
+        return first_order("layer_norm", grads, {want_x ? (shared ? dS : dX) : Tensor(), want_r ? dS : Tensor(), dw, db, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()},
+                           {t != 0, t != 0, (t & 1) != 0});
     }
 };
 
