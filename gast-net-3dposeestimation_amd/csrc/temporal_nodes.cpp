@@ -6,6 +6,7 @@
 #include <dlfcn.h>
 #include <torch/extension.h>
 #include <c10/hip/HIPStream.h>
+#include <c10/core/AutogradState.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include "../../include/gast_hip.h"
@@ -85,6 +86,12 @@ bool records(std::initializer_list<const Tensor*> ts) {
     for (const Tensor* t : ts)
         if (t->defined() && t->requires_grad()) return true;
     return false;
+}
+// Forward-mode derivatives are not there: a tangent would be left behind, which is a derivative of zero.
+void no_tangents(const char* what, std::initializer_list<const Tensor*> ts) {
+    if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+    for (const Tensor* t : ts)
+        TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), what, ": there is no forward-mode derivative");
 }
 Tensor or_none(const optional<Tensor>& t) { return t.has_value() ? *t : Tensor(); }
 optional<Tensor> maybe(const Tensor& t) { return t.defined() ? optional<Tensor>(t) : std::nullopt; }      // (nodes take no undefined inputs)
@@ -180,7 +187,10 @@ struct RotaryNode : torch::autograd::Function<RotaryNode> {
 std::vector<Tensor> rotary(const std::vector<Tensor>& given, Tensor positions, const Tensor& freqs, bool interleaved, double scale) {
     TORCH_CHECK_VALUE(!given.empty() && given.size() <= GAST_ROTARY_MAX_BATCH, "rotary: 1 to ", GAST_ROTARY_MAX_BATCH, " tensors in a call, got ", given.size());
     std::vector<Tensor> xs;
-    for (const Tensor& t : given) xs.push_back(heads("rotary", "x", t));
+    for (const Tensor& t : given) {
+        no_tangents("rotary", {&t, &freqs});
+        xs.push_back(heads("rotary", "x", t));
+    }
     const Tensor& x = xs[0];
     const int64_t B = x.size(0), T = x.size(1), D = x.size(4);
     for (const Tensor& t : xs)
@@ -322,6 +332,7 @@ variable_list decay_attention(const Tensor& q, const Tensor& k, const Tensor& v,
     const char* what = "decay_attention";
     const Tensor Q = heads(what, "q", q), K = heads(what, "k", k), V = heads(what, "v", v);
     Tensor state = or_none(state_), lengths = or_none(lengths_);
+    no_tangents(what, {&q, &k, &v, &log_decay, &state});
     const double scale = decay_check(what, Q, K, V, log_decay, state, lengths, scale_);
     if (state.defined()) state = state.contiguous();
     variable_list out = records({&q, &k, &v, &state}) ? DecayNode::apply(Q, K, V, log_decay, maybe(state), maybe(lengths), scale, return_state)
@@ -336,6 +347,7 @@ Tensor decay_attention_step(const Tensor& q, const Tensor& k, const Tensor& v, T
     TORCH_CHECK_VALUE(q.dim() == k.dim() && q.dim() == v.dim() && (q.dim() == 3 || q.dim() == 4), what, ": q, k and v have to be (B, J, H, D) or (B, H, D), got ",
                       q.sizes(), ", ", k.sizes(), ", ", v.sizes());
     TORCH_CHECK(!records({&q, &k, &v, &state}), what, " updates the state in place and has no gradient: call it under torch.no_grad(), or use decay_attention");
+    no_tangents(what, {&q, &k, &v, &log_decay, &state});
     const Tensor Q = heads(what, "q", q.unsqueeze(1)), K = heads(what, "k", k.unsqueeze(1)), V = heads(what, "v", v.unsqueeze(1));
     Tensor lengths = or_none(lengths_);
     const double scale = decay_check(what, Q, K, V, log_decay, state, lengths, scale_);
@@ -453,6 +465,7 @@ variable_list norm(const std::string& what, const Tensor& x, const optional<Tens
     TORCH_CHECK_VALUE(C > 0 && C <= MAX_AXIS, what, ": x needs a last axis of 1 to ", MAX_AXIS, " values to normalise, got ", x.sizes());
     const Tensor residual = or_none(residual_);
     Tensor weight = or_none(weight_), bias = or_none(bias_), seed = or_none(seed_);
+    no_tangents(what.c_str(), {&x, &residual, &weight, &bias});
     if (residual.defined())
         TORCH_CHECK_VALUE(residual.sizes() == x.sizes() && residual.scalar_type() == x.scalar_type(), what, ": x and residual differ: ", x.sizes(), " ", x.scalar_type(),
                           " and ", residual.sizes(), " ", residual.scalar_type());

@@ -13,7 +13,7 @@ checks, autograd nodes and kernel calls are csrc/temporal_nodes.cpp (gast_hip/_t
 Every call can be captured into a HIP graph (workspaces come from torch's allocator, so every graph has its own), a backward pass together
 with its forward pass, on leaves made for the capture: no graph of the same leaves that was recorded outside the capture may be alive then,
 because autograd would make the capture wait for the stream of the older one.
-There is no second derivative: asking for one raises.
+There is no second derivative and no forward-mode one: asking for one raises.
 """
 import os
 
