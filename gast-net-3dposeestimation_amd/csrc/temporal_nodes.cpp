@@ -314,7 +314,7 @@ double decay_check(const char* what, const Tensor& q, const Tensor& k, const Ten
     TORCH_CHECK_VALUE(std::max(Dk, Dv) <= GAST_DECAY_MAX_D, what, ": at most ", GAST_DECAY_MAX_D, " channels a head, got ", Dk, " and ", Dv);
     TORCH_CHECK_VALUE(log_decay.dim() == 1 && log_decay.size(0) == H && log_decay.is_floating_point(), what, ": log_decay holds one number for each of the ", H,
                       " heads, got ", log_decay.scalar_type(), " ", log_decay.sizes());
-    TORCH_CHECK_VALUE(!log_decay.requires_grad(), what, ": the decays are fixed: there is no gradient for log_decay (pass log_decay.detach())");
+    TORCH_CHECK_VALUE(!records({&log_decay}), what, ": the decays are fixed: there is no gradient for log_decay (pass log_decay.detach())");
     if (state.defined())
         TORCH_CHECK_VALUE(state.sizes() == at::IntArrayRef({B, J, H, Dk, Dv}) && state.scalar_type() == at::kFloat, what, ": the state has to be float32 (", B, ", ",
                           J, ", ", H, ", ", Dk, ", ", Dv, "), got ", state.scalar_type(), " ", state.sizes());

@@ -1,0 +1,27 @@
+"""Calls that the documentation of gast_hip.temporal allows, beside those of sizes and types."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope='module')
+def tp():
+    from gast_hip import temporal
+    return temporal
+
+
+def randn(*shape, seed=0, dtype=torch.float32):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).to(dtype).cuda()
+
+
+def test_inference_with_decays_that_are_a_parameter(tp):
+    q, k, v, s = randn(2, 9, 1, 3, 8, seed=1), randn(2, 9, 1, 3, 8, seed=2), randn(2, 9, 1, 3, 16, seed=3), randn(2, 1, 3, 8, 16, seed=4)
+    ld = torch.nn.Parameter(torch.tensor([-0.1, -0.01, 0.0]).cuda())
+    with torch.no_grad():
+        got = tp.decay_attention(q, k, v, ld, state=s, return_state=True)
+        want = tp.decay_attention(q, k, v, ld.detach(), state=s, return_state=True)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        s1, s2 = s.clone(), s.clone()
+        assert torch.equal(tp.decay_attention_step(q[:, 0], k[:, 0], v[:, 0], ld, s1), tp.decay_attention_step(q[:, 0], k[:, 0], v[:, 0], ld.detach(), s2))
+        assert torch.equal(s1, s2)

@@ -37,3 +37,14 @@ def test_tangents_are_refused(name, grad):
             t[n] = fwAD.unpack_dual(t[n]).primal
             with pytest.raises(RuntimeError, match='no CPU fallback'):          # (and goes on without one)
                 call(t)
+
+
+@pytest.mark.parametrize('name', ['decay_attention', 'decay_attention_step'])
+def test_a_trained_decay_is_refused_only_where_autograd_records(name):
+    """inference of a model that holds its decays as a parameter"""
+    t = inputs()
+    t['log_decay'].requires_grad_(True)
+    with pytest.raises(ValueError, match='no gradient for log_decay'):
+        CALLS[name][0](t)
+    with torch.no_grad(), pytest.raises(RuntimeError, match='no CPU fallback'):
+        CALLS[name][0](t)
