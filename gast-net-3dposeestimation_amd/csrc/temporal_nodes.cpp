@@ -198,6 +198,7 @@ std::vector<Tensor> rotary(const std::vector<Tensor>& given, Tensor positions, c
                           "rotary: tensors of one call differ in their heads alone, got ", x.sizes(), " ", x.scalar_type(), " and ", t.sizes(), " ", t.scalar_type());
     TORCH_CHECK_VALUE(freqs.dim() == 1 && freqs.scalar_type() == at::kDouble && freqs.size(0) >= 1 && freqs.size(0) <= D / 2,
                       "rotary: freqs is a float64 vector of 1 to ", D / 2, " frequencies, got ", freqs.scalar_type(), " ", freqs.sizes());
+    TORCH_CHECK_VALUE(!records({&freqs}), "rotary: the frequencies are fixed: there is no gradient for freqs (pass freqs.detach())");
     TORCH_CHECK_VALUE(D <= GAST_ROTARY_MAX_D, "rotary: at most ", GAST_ROTARY_MAX_D, " channels a head, got ", D);
     TORCH_CHECK_VALUE(positions.scalar_type() == at::kInt || positions.scalar_type() == at::kLong, "rotary: positions are int32 or int64, got ", positions.scalar_type());
     if (positions.dim() == 1 && positions.size(0) == T) positions = positions.unsqueeze(0);

@@ -62,7 +62,8 @@ def rotary(x, positions, freqs, interleaved=False, scale=1.0):
     """x with the first 2 * len(freqs) channels of every head turned by positions * freqs and multiplied by `scale`, the others as they
     are.  x: one tensor, or a tuple of up to four (q and k, say, with heads of their own) that are turned in one launch.  Pairs are
     channels (f, f + len(freqs)), or (2 f, 2 f + 1) with interleaved=True.  positions: (T,) for all clips or (B, T), int32 or int64, any
-    values (angles are reduced in 64 bits).  Differentiable in x."""
+    values (angles are reduced in 64 bits).  Differentiable in x; freqs that require grad
+    are refused where autograd records."""
     if isinstance(x, (tuple, list)):
         return tuple(_temporal.rotary(x, positions, freqs, interleaved, scale))
     return _temporal.rotary((x,), positions, freqs, interleaved, scale)[0]

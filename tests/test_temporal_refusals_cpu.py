@@ -48,3 +48,13 @@ def test_a_trained_decay_is_refused_only_where_autograd_records(name):
         CALLS[name][0](t)
     with torch.no_grad(), pytest.raises(RuntimeError, match='no CPU fallback'):
         CALLS[name][0](t)
+
+
+def test_trained_frequencies_are_refused_where_autograd_records():
+    """they got no gradient, without a word"""
+    t = inputs()
+    t['freqs'].requires_grad_(True)
+    with pytest.raises(ValueError, match='no gradient for freqs'):
+        CALLS['rotary'][0](t)
+    with torch.no_grad(), pytest.raises(RuntimeError, match='no CPU fallback'):
+        CALLS['rotary'][0](t)
