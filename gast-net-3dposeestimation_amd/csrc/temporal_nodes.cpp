@@ -350,9 +350,9 @@ Tensor decay_attention_step(const Tensor& q, const Tensor& k, const Tensor& v, T
     TORCH_CHECK(!records({&q, &k, &v, &state}), what, " updates the state in place and has no gradient: call it under torch.no_grad(), or use decay_attention");
     no_tangents(what, {&q, &k, &v, &log_decay, &state});
     const Tensor Q = heads(what, "q", q.unsqueeze(1)), K = heads(what, "k", k.unsqueeze(1)), V = heads(what, "v", v.unsqueeze(1));
+    TORCH_CHECK_VALUE(state.is_contiguous(), what, ": the state has to be contiguous, got strides ", state.strides(), " of ", state.sizes());
     Tensor lengths = or_none(lengths_);
     const double scale = decay_check(what, Q, K, V, log_decay, state, lengths, scale_);
-    TORCH_CHECK_VALUE(state.is_contiguous(), what, ": the state has to be contiguous");
     const Tensor o = fresh(V);
     if (q.size(0)) {
         const Here here(q);

@@ -25,3 +25,17 @@ def test_inference_with_decays_that_are_a_parameter(tp):
         s1, s2 = s.clone(), s.clone()
         assert torch.equal(tp.decay_attention_step(q[:, 0], k[:, 0], v[:, 0], ld, s1), tp.decay_attention_step(q[:, 0], k[:, 0], v[:, 0], ld.detach(), s2))
         assert torch.equal(s1, s2)
+
+
+def test_a_step_leaves_a_strided_state_alone(tp):
+    q, k, v = randn(2, 1, 2, 4, seed=1), randn(2, 1, 2, 4, seed=2), randn(2, 1, 2, 5, seed=3)
+    buf = randn(2, 1, 2, 5, 4, seed=4)
+    was = buf.clone()
+    with pytest.raises(ValueError, match='has to be contiguous'):
+        tp.decay_attention_step(q, k, v, torch.zeros(2).cuda(), buf.transpose(3, 4))
+    assert torch.equal(buf, was)
+    wide = randn(2, 1, 2, 4, 10, seed=5)
+    was = wide.clone()
+    with pytest.raises(ValueError, match='has to be contiguous'):
+        tp.decay_attention_step(q, k, v, torch.zeros(2).cuda(), wide[..., ::2])
+    assert torch.equal(wide, was)

@@ -58,3 +58,16 @@ def test_trained_frequencies_are_refused_where_autograd_records():
         CALLS['rotary'][0](t)
     with torch.no_grad(), pytest.raises(RuntimeError, match='no CPU fallback'):
         CALLS['rotary'][0](t)
+
+
+def strided_states():
+    """states of the right size whose numbers do not lie one after the other"""
+    return [z(2, 1, 2, 5, 4).transpose(3, 4), z(2, 1, 2, 4, 10)[..., ::2], z(1, 1, 2, 4, 5).expand(2, 1, 2, 4, 5), z(4, 1, 2, 4, 5)[::2]]
+
+
+@pytest.mark.parametrize('i', range(4))
+def test_a_step_refuses_a_state_that_is_not_contiguous(i):
+    t = dict(inputs(), state=strided_states()[i])
+    assert t['state'].shape == (2, 1, 2, 4, 5)
+    with pytest.raises(ValueError, match='has to be contiguous'):
+        CALLS['decay_attention_step'][0](t)
