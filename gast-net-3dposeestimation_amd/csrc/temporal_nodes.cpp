@@ -467,6 +467,7 @@ variable_list norm(const std::string& what, const Tensor& x, const optional<Tens
     const Tensor residual = or_none(residual_);
     Tensor weight = or_none(weight_), bias = or_none(bias_), seed = or_none(seed_);
     no_tangents(what.c_str(), {&x, &residual, &weight, &bias});
+    TORCH_CHECK_VALUE(residual.defined() || what != "add_layer_norm", what, ": a residual is needed (layer_norm goes without)");
     if (residual.defined())
         TORCH_CHECK_VALUE(residual.sizes() == x.sizes() && residual.scalar_type() == x.scalar_type(), what, ": x and residual differ: ", x.sizes(), " ", x.scalar_type(),
                           " and ", residual.sizes(), " ", residual.scalar_type());

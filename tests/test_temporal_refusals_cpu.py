@@ -71,3 +71,9 @@ def test_a_step_refuses_a_state_that_is_not_contiguous(i):
     assert t['state'].shape == (2, 1, 2, 4, 5)
     with pytest.raises(ValueError, match='has to be contiguous'):
         CALLS['decay_attention_step'][0](t)
+
+
+def test_add_layer_norm_needs_a_residual():
+    """it returned one output instead of two"""
+    with pytest.raises(ValueError, match='add_layer_norm: a residual is needed'):
+        tp.add_layer_norm(z(2, 4), None)
