@@ -547,7 +547,7 @@ __global__ void __launch_bounds__((Lay<T, DP, MODE>::NT), (STATE ? 2 : 4)) chunk
     if (nchunk) fetch(c_first);
     Powers& pw = m.pw;
     if (tid <= CT) {
-        const float p = power(lg, (float)tid);
+        const float p = tid <= count ? power(lg, (float)tid) : 0.f;         // (a growing one may overflow where there are no tokens: no inf times 0)
         pw.up[tid] = p;
         if constexpr (STATE) {
             const float u = power(lg, 32.f * tid);

@@ -74,9 +74,9 @@ def decay_attention(q, k, v, log_decay, state=None, lengths=None, scale=None, re
     """Causal linear attention with a decay for each head:  S_t = exp(log_decay[h]) S_(t-1) + k_t v_t',  o_t = scale q_t' S_t.
 
     q, k: (B, T, J, H, Dk), v: (B, T, J, H, Dv), or without J; at most 128 channels a head.  Heads shared by several query heads are
-    passed expanded (a stride of 0 is read as it is).  log_decay: (H,), normally <= 0 (minus infinity: no memory), not trained
-    (one that requires grad is refused where autograd records).  state:
-    S before the first token, (B, J, H, Dk, Dv) float32 (J = 1 for plain sequences; None: zero).  lengths: (B,) tokens of each clip,
+    passed expanded (a stride of 0 is read as it is).  log_decay: (H,), normally <= 0 (minus infinity: no memory; above 0
+    exp(log_decay * min(tokens, 32)) has to be a finite fp32 number), not trained: one that requires grad is refused where autograd records.
+    state: S before the first token, (B, J, H, Dk, Dv) float32 (J = 1 for plain sequences; None: zero).  lengths: (B,) tokens of each clip,
     clamped to 0 .. T (None: T); outputs and gradients behind a clip's end are zero, whatever stands there in the inputs.  scale: Dk ** -0.5.
     Returns o, or (o, state behind the last token of each clip) with return_state=True.  Differentiable in q, k, v and state; S is held in
     fp32 throughout."""

@@ -1,6 +1,7 @@
 """Calls that the documentation of gast_hip.temporal allows, beside those of sizes and types."""
 import pytest
 import torch
+from test_temporal_gpu import check_decay, decay_case
 
 pytestmark = pytest.mark.gpu
 
@@ -39,3 +40,15 @@ def test_a_step_leaves_a_strided_state_alone(tp):
     with pytest.raises(ValueError, match='has to be contiguous'):
         tp.decay_attention_step(q, k, v, torch.zeros(2).cuda(), wide[..., ::2])
     assert torch.equal(wide, was)
+
+
+@pytest.mark.parametrize('dt', [torch.float32, torch.bfloat16], ids=['fp32', 'bf16'])
+@pytest.mark.parametrize('T,grows', [(1, [5.0]), (2, [10.0, 5.0]), (7, [5.0, -0.1]), (20, [4.0, 3.0]), (27, [3.0])])
+@pytest.mark.parametrize('D', [16, 72])
+def test_strongly_growing_states_of_short_sequences(tp, dt, T, grows, D):
+    """lambda^31 is no fp32 number, but nobody is 31 tokens away (tolerances: decay_tol; binary16 cannot hold the results)"""
+    for state in (False, True):
+        check_decay(tp, decay_case(T, dt, 2, T, 1, 2, D, D, state=state, decays=grows))
+    c = decay_case(T, dt, 3, 100, 1, 2, D, D, decays=grows)
+    c['lengths'] = torch.tensor([T, T // 2, 0], dtype=torch.int32)
+    check_decay(tp, c)
