@@ -255,7 +255,14 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) norm_bwd_kernel(const NormA
         if constexpr (ADD)
 #pragma unroll
             for (int i = 0; i < NC; ++i) ldv<VE>(st[i], (const T*)a.dSt + in * a.ldds + at[i]);
-        const float mean = a.mean[in], rstd = a.rstd[in];
+        float mean = a.mean[in], rstd = a.rstd[in];
+        if (!a.dY) {                                     // (the stream's gradient passes as it is, in rows with infinities too)
+            mean = rstd = 0.f;
+#pragma unroll
+            for (int i = 0; i < NC; ++i)
+#pragma unroll
+                for (int e = 0; e < VE; ++e) h[i][e] = 0.f;
+        }
         if (!on || nvec < NC * G || !a.dY)
 #pragma unroll
             for (int i = 0; i < NC; ++i)
@@ -333,10 +340,10 @@ __global__ void __launch_bounds__(1024) norm_bwd_long_kernel(const NormArgs a) {
     for (long row = blockIdx.x; row < a.rows; row += gridDim.x, par ^= 1, first = false) {
         const T* s = (const T*)a.S + row * a.lds;
         const T* dy = a.dY ? (const T*)a.dY + row * a.lddy : nullptr;
-        const float mean = a.mean[row], rstd = a.rstd[row];
+        const float mean = dy ? a.mean[row] : 0.f, rstd = dy ? a.rstd[row] : 0.f;       // (without dY nothing of the row counts, infinities neither)
         float t0 = 0.f, t1 = 0.f;
         for (int c = threadIdx.x; c < C; c += 1024) {
-            const float y = dy ? Elem<T>::ld(dy + c) : 0.f, h = (Elem<T>::ld(s + c) - mean) * rstd, g = a.gamma ? y * a.gamma[c] : y;
+            const float y = dy ? Elem<T>::ld(dy + c) : 0.f, h = dy ? (Elem<T>::ld(s + c) - mean) * rstd : 0.f, g = a.gamma ? y * a.gamma[c] : y;
             if (out) {                                   // (this block's partial row; column c belongs to this thread alone)
                 out[c] = first ? y * h : fmaf(y, h, out[c]);
                 out[C + c] = first ? y : out[C + c] + y;
@@ -347,7 +354,7 @@ __global__ void __launch_bounds__(1024) norm_bwd_long_kernel(const NormArgs a) {
         t0 = group_sum<1024>(t0, red[par][0]) * inv;
         t1 = group_sum<1024>(t1, red[par][1]) * inv;
         for (int c = threadIdx.x; c < C; c += 1024) {
-            const float y = dy ? Elem<T>::ld(dy + c) : 0.f, h = (Elem<T>::ld(s + c) - mean) * rstd, g = a.gamma ? y * a.gamma[c] : y;
+            const float y = dy ? Elem<T>::ld(dy + c) : 0.f, h = dy ? (Elem<T>::ld(s + c) - mean) * rstd : 0.f, g = a.gamma ? y * a.gamma[c] : y;
             float d = fmaf(rstd, g - t0 - h * t1, a.dSt ? Elem<T>::ld((const T*)a.dSt + row * a.ldds + c) : 0.f);
             if (a.dS) Elem<T>::st((T*)a.dS + row * a.lddsum + c, d);
             if (a.dX) {

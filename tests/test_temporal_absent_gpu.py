@@ -59,3 +59,21 @@ def test_the_other_operators_without_a_gradient(tp):
     f = tp.rotary_frequencies(8).cuda()
     nothing((tp.rotary(q, torch.arange(40).cuda(), f),), [q])
     nothing(tp.rotary((q, k), torch.arange(40).cuda(), f), [q, k])
+
+
+@pytest.mark.parametrize('dt', [torch.float32, torch.bfloat16, torch.float16], ids=['fp32', 'bf16', 'fp16'])
+@pytest.mark.parametrize('C', [7, 32, 130, 4096, 20000])
+@pytest.mark.parametrize('p', [0.0, 0.5])
+def test_the_streams_gradient_alone_passes_rows_with_infinities(tp, dt, C, p):
+    """where nobody differentiates y, the norm of such a row (NaN) has no part in anything"""
+    from gast_hip.binding import Dropout, dropout_params
+    drop = Dropout(torch.tensor([3], dtype=torch.int32).cuda(), *dropout_params(p)) if p else None
+    x, r, w, b = (t.detach().to(d).requires_grad_(True) for t, d in ((leaf(9, C), dt), (leaf(9, C), dt), (leaf(C), torch.float32), (leaf(C), torch.float32)))
+    with torch.no_grad():
+        r[2, C // 2], r[8, 0], r[5, C - 1] = float('inf'), float('nan'), -float('inf')
+    y, s = tp.add_layer_norm(x, r, w, b, drop=drop)
+    ds = leaf(9, C + 1)[:, :C].detach().to(dt)
+    dx, dr, dw, db = torch.autograd.grad(Mute.apply(y) + (s * ds).sum(), [x, r, w, b], allow_unused=True)
+    assert torch.equal(dr, ds)
+    assert torch.isfinite(dx).all() and (p or torch.equal(dx, ds))
+    assert not dw.any() and not db.any()
