@@ -278,6 +278,8 @@ struct DecayNode : torch::autograd::Function<DecayNode> {
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const auto s = ctx->get_saved_variables();
         const Tensor &q = s[0], &k = s[1], &v = s[2], &state = s[4];
+        const bool only_state = !grads[0].defined();
+        if (only_state && (grads.size() < 2 || !grads[1].defined())) return variable_list(8);
         const Tensor dq = fresh(q), dk = fresh(k), dv = fresh(v);
         Tensor dstate, dnext = grads.size() > 1 ? grads[1] : Tensor();
         if (state.defined() && ctx->needs_input_grad(4)) dstate = fresh(state);
@@ -285,8 +287,15 @@ struct DecayNode : torch::autograd::Function<DecayNode> {
         if (q.size(0) * q.size(1) > 0) {
             const Here here(q);
             const Lib& l = lib(q.scalar_type());
-            const Tensor d_o = grads[0].defined() ? last_contiguous(grads[0]) : at::zeros(v.sizes(), v.options());
-            gast_decay_args a = decay_args(q, k, v, s[3], state, s[5], ctx->saved_data["scale"].toDouble());
+            Tensor d_o, queries = q;
+            if (only_state) {              // the state does not see the queries, infinities among them neither: one row of zeros stands for all
+                const Tensor none = at::zeros({GAST_DECAY_MAX_D}, v.options());
+                d_o = none.narrow(0, 0, v.size(4)).expand(v.sizes());
+                queries = none.narrow(0, 0, q.size(4)).expand(q.sizes());
+            } else {
+                d_o = last_contiguous(grads[0]);
+            }
+            gast_decay_args a = decay_args(queries, k, v, s[3], state, s[5], ctx->saved_data["scale"].toDouble());
             a.d_o = seq(d_o); a.dq = seq(dq); a.dk = seq(dk); a.dv = seq(dv);
             a.dstate_out = f32(dnext);
             a.dstate = f32(dstate);
@@ -300,7 +309,8 @@ struct DecayNode : torch::autograd::Function<DecayNode> {
         // (the outputs are linear in each input: a gradient is made from the others)
         const int64_t t = ctx->saved_data["trained"].toInt();
         const bool tq = t & 1, tk = t & 2, tv = t & 4, ts = t & 8;
-        return first_order("decay_attention", grads, {dq, dk, dv, Tensor(), dstate, Tensor(), Tensor(), Tensor()}, {tk || tv || ts, tq || tv, tq || tk, false, tq});
+        return first_order("decay_attention", grads, {only_state ? Tensor() : dq, dk, dv, Tensor(), dstate, Tensor(), Tensor(), Tensor()},
+                           {tk || tv || ts, tq || tv, tq || tk, false, tq});
     }
 };
 

@@ -77,3 +77,22 @@ def test_the_streams_gradient_alone_passes_rows_with_infinities(tp, dt, C, p):
     assert torch.equal(dr, ds)
     assert torch.isfinite(dx).all() and (p or torch.equal(dx, ds))
     assert not dw.any() and not db.any()
+
+
+@pytest.mark.parametrize('dt', [torch.float32, torch.bfloat16, torch.float16], ids=['fp32', 'bf16', 'fp16'])
+@pytest.mark.parametrize('T,Dk,Dv', [(1, 8, 8), (20, 3, 40), (40, 32, 16), (70, 100, 128), (2000, 16, 24)])
+def test_the_states_gradient_alone_does_not_see_the_queries(tp, dt, T, Dk, Dv):
+    q, k, v = (t.detach().to(dt) for t in (leaf(2, T, 1, 2, Dk), leaf(2, T + 1, 1, 2, Dk)[:, :T], leaf(2, T, 1, 2, Dv)))
+    s, dn = leaf(2, 1, 2, Dk, Dv).detach(), leaf(2, 1, 2, Dk, Dv).detach()
+    ld = torch.tensor([-0.1, -0.01], device='cuda')
+    wild = q.clone()
+    wild[0, T // 2, 0, 1, 0], wild[1, 0, 0, 0, Dk - 1] = float('nan'), float('inf')
+    got = []
+    for queries, zero in ((q, True), (q, False), (wild, False)):
+        t = [x.clone().requires_grad_(True) for x in (queries, k, v, s)]
+        o, new = tp.decay_attention(*t[:3], ld, state=t[3], return_state=True)
+        outs, grads = ([o, new], [torch.zeros_like(o), dn]) if zero else ([new], [dn])
+        got.append(torch.autograd.grad(outs, t, grads, allow_unused=True))
+    for name, a, b, c in zip(('dk', 'dv', 'dstate'), *(g[1:] for g in got)):
+        assert torch.equal(a, b) and torch.equal(b, c), name
+    assert all(g[0] is None or not g[0].any() for g in got)
