@@ -508,7 +508,8 @@ __global__ void __launch_bounds__((Lay<T, DP, MODE>::NT), (STATE ? 2 : 4)) chunk
     const int ia = BWD ? (grp == 0 ? 2 : grp == 1 ? 3 : 1) : 0, ib = BWD ? (grp == 0 ? 0 : grp == 1 ? 1 : 3) : 1, ic = BWD ? (grp == 0 ? 1 : grp == 1 ? 0 : 2) : 2;
     // offsets in a set of tiles: rows, and columns of turned tiles or of rows
     constexpr int COL0 = L::TURNED ? TURN0 : MODE == ONE ? L::ROWS : 0, CS = L::TURNED ? TS : 1;       // (the columns of b of ONE and SUMS; a column's step)
-    const int oa = ia * L::ROWS, ob = ib * L::ROWS, obT = COL0 + (BWD ? ib : 0) * L::TURN;
+    // (v has no turned tile: the dq waves of THREE hand no state on, and make theirs of k)
+    const int oa = ia * L::ROWS, ob = ib * L::ROWS, obT = COL0 + (BWD ? (L::TURNED ? min(ib, 2) : ib) : 0) * L::TURN;
     const int oc = COL0 + (BWD ? ic : 1) * L::TURN + wv * 32 * CS;                                // (this wave's 32 columns of c)
     const int c0 = wv * 32 + col, D1 = ro.D1, D2 = ro.D2;
     const bool works = wv * 32 < D2;

@@ -52,3 +52,14 @@ def test_strongly_growing_states_of_short_sequences(tp, dt, T, grows, D):
     c = decay_case(T, dt, 3, 100, 1, 2, D, D, decays=grows)
     c['lengths'] = torch.tensor([T, T // 2, 0], dtype=torch.int32)
     check_decay(tp, c)
+
+
+@pytest.mark.parametrize('dt', [torch.float32, torch.bfloat16, torch.float16], ids=['fp32', 'bf16', 'fp16'])
+@pytest.mark.parametrize('T,Dk,Dv', [(1, 32, 32), (27, 64, 64), (32, 48, 16), (9, 3, 64), (31, 33, 5), (5, 1, 1)])
+def test_sequences_of_one_chunk_that_go_on_from_a_state(tp, dt, T, Dk, Dv):
+    """their backward pass is one launch whose waves share their tiles"""
+    c = decay_case(T, dt, 7, T, 2, 3, Dk, Dv, ragged=True)
+    first = check_decay(tp, c)
+    for _ in range(3):
+        again = check_decay(tp, c)
+        assert all(torch.equal(first[n], again[n]) for n in first)
