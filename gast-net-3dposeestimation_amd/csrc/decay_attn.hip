@@ -26,9 +26,10 @@ namespace {
 // LDS round trip.
 //
 // Arithmetic.  fp32: fp32 matrix instructions.  16 bits: products of stored values are exact in fp32; scores and states, which are fp32,
-// meet 16-bit operands as two bf16 parts (hi = bf16(x), lo = bf16(x - hi): 2^-17 relative), what enters a state as three (all 24 bits: states
-// are results in fp32); in the binary16 flavour the stored operand is split into two bf16 parts as well (exactly; binary16 parts of a state
-// would overflow at 65504).  States are fp32 throughout.
+// meet 16-bit operands as three bf16 parts that hold all of their 24 bits; in the binary16 flavour the stored operand is split into two bf16
+// parts as well (exactly; binary16 parts of a state would overflow at 65504).  So the 16-bit types compute as fp32 does, and only results are
+// rounded to the type.  Two parts (2^-17 of each score and state) are faster, 8 - 21 % with 128 channels a head (512 heads, 1024 tokens, bf16: 154
+// against 183 us, with gradients 585 against 705), 5 - 14 % with 64, but what is left of terms that nearly cancel is then off by 2^-17 of the terms.
 //
 // What bounds it, on a full card (two waves a SIMD, 1024 tokens, without gradients; a copy of the same bytes takes 112 us at 16 bits, 224 fp32):
 //   bf16  1024 heads of 64: 128 us, memory (4.2 TB/s); 512 of 128: 145 us, issue (586 vector, 52 matrix and 54 LDS instructions a wave and chunk:
@@ -42,8 +43,7 @@ constexpr int TS = CT + 4;           // row pitch of the turned tiles (elements)
 template <typename T> struct Frag;
 template <> struct Frag<float> { float x[16]; };
 template <> struct Frag<bf16_t> { uint4 x[2]; };
-struct Split { uint4 hi[2], lo[2]; };                  // x = hi + lo to 2^-17
-struct Parts { uint4 x[3][2]; };                       // x = x[0] + x[1] + x[2], all of its 24 bits
+struct Parts { uint4 x[3][2]; };                       // x = x[0] + x[1] + x[2], bf16 parts that hold all of its 24 bits
 
 // 16 values of a row of an LDS tile: elements 8 q + 4 (lane / 32) + 0 .. 3, q = 0 .. 3
 __device__ __forceinline__ Frag<float> ld_frag(const float* row, int half) {
@@ -91,20 +91,20 @@ __device__ __forceinline__ uint32_t take2(float& a, float& b) {
     b -= __uint_as_float(u & 0xffff0000u);
     return u;
 }
-template <typename V> __device__ __forceinline__ Split split16(const V& v) {
-    Split s;
+template <typename V> __device__ __forceinline__ Parts parts16(const V& v) {
+    Parts s;
+    float w[16];
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-        uint32_t h[4], l[4];
+    for (int i = 0; i < 16; ++i) w[i] = v[i];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            float a = v[8 * q + 2 * e], b = v[8 * q + 2 * e + 1];
-            h[e] = take2(a, b);
-            l[e] = pack_bf16x2(a, b);
+    for (int k = 0; k < 3; ++k)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            uint32_t u[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) u[e] = take2(w[8 * q + 2 * e], w[8 * q + 2 * e + 1]);
+            s.x[k][q] = make_uint4(u[0], u[1], u[2], u[3]);
         }
-        s.hi[q] = make_uint4(h[0], h[1], h[2], h[3]);
-        s.lo[q] = make_uint4(l[0], l[1], l[2], l[3]);
-    }
     return s;
 }
 
@@ -126,69 +126,70 @@ template <typename V> __device__ __forceinline__ void mma_sf(f32x16& c, const Fr
 #pragma unroll
     for (int i = 0; i < 16; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.x[i], b[i], c, 0, 0, 0);
 }
-__device__ __forceinline__ Split stored_parts(const Frag<bf16_t>& f) {
-    float v[16];
-    unpack(f, v);
-    return split16(v);
-}
-__device__ __forceinline__ void mma_fs(f32x16& c, const Split& a, const Frag<bf16_t>& b) {
 #ifdef GAST_H16_F16
-    const Split p = stored_parts(b);
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-        c = mfma_pair<1>(a.lo[q], p.hi[q], c);
-        c = mfma_pair<1>(a.hi[q], p.lo[q], c);
-        c = mfma_pair<1>(a.hi[q], p.hi[q], c);
-    }
-#else
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-        c = mfma_pair<1>(a.lo[q], b.x[q], c);
-        c = mfma_pair<1>(a.hi[q], b.x[q], c);
-    }
-#endif
-}
-__device__ __forceinline__ void mma_sf(f32x16& c, const Frag<bf16_t>& a, const Split& b) {
-#ifdef GAST_H16_F16
-    const Split p = stored_parts(a);
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-        c = mfma_pair<1>(p.hi[q], b.lo[q], c);
-        c = mfma_pair<1>(p.lo[q], b.hi[q], c);
-        c = mfma_pair<1>(p.hi[q], b.hi[q], c);
-    }
-#else
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-        c = mfma_pair<1>(a.x[q], b.lo[q], c);
-        c = mfma_pair<1>(a.x[q], b.hi[q], c);
-    }
-#endif
-}
-template <typename V> __device__ __forceinline__ Parts parts16(const V& v) {
-    Parts s;
-    float w[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) w[i] = v[i];
-#pragma unroll
-    for (int k = 0; k < 3; ++k)
+// a binary16 value is two bf16 parts (exactly)
+struct Stored {
+    uint4 hi[2], lo[2];
+    __device__ __forceinline__ explicit Stored(const Frag<bf16_t>& f) {
+        float v[16];
+        unpack(f, v);
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-            uint32_t u[4];
+            uint32_t h[4], l[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                u[e] = take2(w[8 * q + 2 * e], w[8 * q + 2 * e + 1]);
+                h[e] = take2(v[8 * q + 2 * e], v[8 * q + 2 * e + 1]);
+                l[e] = pack_bf16x2(v[8 * q + 2 * e], v[8 * q + 2 * e + 1]);
             }
-            s.x[k][q] = make_uint4(u[0], u[1], u[2], u[3]);
+            hi[q] = make_uint4(h[0], h[1], h[2], h[3]);
+            lo[q] = make_uint4(l[0], l[1], l[2], l[3]);
         }
-    return s;
+    }
+};
+#endif
+// (the product of the smallest parts of both sides, 2^-24 of a term, is left out)
+__device__ __forceinline__ void mma_fs(f32x16& c, const Parts& a, const Frag<bf16_t>& b) {
+#ifdef GAST_H16_F16
+    const Stored p(b);
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        c = mfma_pair<1>(a.x[2][q], p.hi[q], c);
+        c = mfma_pair<1>(a.x[1][q], p.lo[q], c);
+        c = mfma_pair<1>(a.x[1][q], p.hi[q], c);
+        c = mfma_pair<1>(a.x[0][q], p.lo[q], c);
+        c = mfma_pair<1>(a.x[0][q], p.hi[q], c);
+    }
+#else
+#pragma unroll
+    for (int k = 2; k >= 0; --k)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) c = mfma_pair<1>(a.x[k][q], b.x[q], c);
+#endif
+}
+__device__ __forceinline__ void mma_sf(f32x16& c, const Frag<bf16_t>& a, const Parts& b) {
+#ifdef GAST_H16_F16
+    const Stored p(a);
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        c = mfma_pair<1>(p.hi[q], b.x[2][q], c);
+        c = mfma_pair<1>(p.lo[q], b.x[1][q], c);
+        c = mfma_pair<1>(p.hi[q], b.x[1][q], c);
+        c = mfma_pair<1>(p.lo[q], b.x[0][q], c);
+        c = mfma_pair<1>(p.hi[q], b.x[0][q], c);
+    }
+#else
+#pragma unroll
+    for (int k = 2; k >= 0; --k)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) c = mfma_pair<1>(a.x[q], b.x[k][q], c);
+#endif
 }
 // X[q] += A[q] B for every q (bf16: one after the other, so that none waits for the one before)
 template <int G> __device__ __forceinline__ void mma_into(f32x16 (&X)[G], const Frag<bf16_t> (&a)[G], const Parts& b) {
 #ifdef GAST_H16_F16
 #pragma unroll
     for (int q = 0; q < G; ++q) {
-        const Split p = stored_parts(a[q]);
+        const Stored p(a[q]);
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             X[q] = mfma_pair<1>(p.hi[s], b.x[2][s], X[q]);
@@ -207,7 +208,7 @@ template <int G> __device__ __forceinline__ void mma_into(f32x16 (&X)[G], const 
             for (int q = 0; q < G; ++q) X[q] = mfma_pair<1>(a[q].x[s], b.x[k][s], X[q]);
 #endif
 }
-// the fp32 side of mma_sf, prepared once where several products share it: scores in two parts, what enters a state in three
+// the fp32 side of a product, prepared once where several products share it
 template <typename T> struct Prepared;
 template <> struct Prepared<float> {
     float v[16];
@@ -216,9 +217,7 @@ template <> struct Prepared<float> {
         for (int i = 0; i < 16; ++i) v[i] = x[i];
     }
 };
-template <> struct Prepared<bf16_t> { Split v; template <typename V> __device__ __forceinline__ void set(const V& x) { v = split16(x); } };
-template <typename T> struct Exact : Prepared<float> {};
-template <> struct Exact<bf16_t> { Parts v; __device__ __forceinline__ void set(const float (&x)[16]) { v = parts16(x); } };
+template <> struct Prepared<bf16_t> { Parts v; template <typename V> __device__ __forceinline__ void set(const V& x) { v = parts16(x); } };
 
 // Infinities and NaN among stored values: whether there are any; c += where they stand (ones) times which tokens are seen (sees(i): element i);
 // c += A B with zeros in their place.  These run for chunks that hold some; the fences keep their operands from being made all at once, for
@@ -263,7 +262,7 @@ template <typename F> __device__ __forceinline__ void mma_wild(f32x16& c, const 
         __builtin_amdgcn_sched_barrier(0);
     }
 }
-__device__ __forceinline__ void mma_tame(f32x16& c, const Frag<bf16_t>& f, const Split& b) {
+__device__ __forceinline__ void mma_tame(f32x16& c, const Frag<bf16_t>& f, const Parts& b) {
     auto tame = [](uint32_t x) { return x & ~((wild2(x) >> 15) * 0xffffu); };
     Frag<bf16_t> t;
 #pragma unroll
@@ -605,7 +604,7 @@ __global__ void __launch_bounds__((Lay<T, DP, MODE>::NT), (STATE ? 2 : 4)) chunk
             f32x16 P = {}, Y = {};
             const Frag<T> fc = ld_column<RS>(tc + col * CS, half);
             Frag<T> fk[G];
-            Exact<T> pv;
+            Prepared<T> pv;
             auto enter = [&] {                             // c as it enters the state, and the other side of that product
                 if constexpr (AHEAD)
 #pragma unroll
