@@ -28,8 +28,8 @@ namespace {
 // Arithmetic.  fp32: fp32 matrix instructions.  16 bits: products of stored values are exact in fp32; scores and states, which are fp32,
 // meet 16-bit operands as three bf16 parts that hold all of their 24 bits; in the binary16 flavour the stored operand is split into two bf16
 // parts as well (exactly; binary16 parts of a state would overflow at 65504).  So the 16-bit types compute as fp32 does, and only results are
-// rounded to the type.  Two parts (2^-17 of each score and state) are faster, 8 - 21 % with 128 channels a head (512 heads, 1024 tokens, bf16: 154
-// against 183 us, with gradients 585 against 705), 5 - 14 % with 64, but what is left of terms that nearly cancel is then off by 2^-17 of the terms.
+// rounded to the type.  Two parts (2^-17 of each score and state) are faster, 15 - 17 % with 128 channels a head (512 heads, 1024 tokens, bf16: 154
+// against 183 us, with gradients 585 against 705), 5 - 12 % with 64, but what is left of terms that nearly cancel is then off by 2^-17 of the terms.
 //
 // What bounds it, on a full card (two waves a SIMD, 1024 tokens, without gradients; a copy of the same bytes takes 112 us at 16 bits, 224 fp32):
 //   bf16  1024 heads of 64: 128 us, memory (4.2 TB/s); 512 of 128: 145 us, issue (586 vector, 52 matrix and 54 LDS instructions a wave and chunk:

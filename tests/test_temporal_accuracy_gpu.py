@@ -7,6 +7,7 @@ for each, of at most 2 m: 14 * 2 u * 2 m = 56 u m; the result is rounded to its 
 state is 2^-17 = 128 u of each term."""
 import pytest
 import torch
+from test_temporal_gpu import check_decay, decay_case, half
 
 pytestmark = pytest.mark.gpu
 
@@ -95,3 +96,23 @@ def test_states_that_cancel(tp, dt, at, T, D):
     near(attend(tp, (zero, zero, zero), ones, state=turned)['dq'][at], ref, m, dt, 'dq')
     near(attend(tp, (zero, ones, zero), zero, dstate=S)['dv'][at], ref, m, dt, 'dv')
     near(attend(tp, (zero, zero, ones), zero, dstate=turned)['dk'][at], ref, m, dt, 'dk')
+
+
+def fp32_tol(name, ref, mag, c):
+    """decay_tol's bound for fp32 (n = 4 T + Dk + Dv + 64 roundings of u) whatever the type, results rounded to theirs once"""
+    T, Dk, Dv = c['q'].shape[1], c['q'].shape[4], c['v'].shape[4]
+    tol = (4 * T + Dk + Dv + 64) * U * mag[name]
+    if name in ('state', 'dstate0'):
+        return tol + 1e-37
+    h, tiny = half(c['q'].dtype)
+    return tol + h * (ref[name].abs() + tol) + tiny
+
+
+@pytest.mark.parametrize('dt', TYPES, ids=IDS)
+@pytest.mark.parametrize('B,T,H,Dk,Dv', [(2, 1, 2, 2, 64), (2, 3, 2, 1, 128), (3, 27, 4, 4, 32), (2, 33, 2, 2, 16), (2, 70, 3, 17, 33), (1, 130, 2, 128, 128), (3, 65, 1, 64, 96),
+                                         (1, 530, 3, 16, 16), (2, 362, 2, 64, 48), (1, 2050, 1, 8, 128)])
+def test_16_bits_meet_the_bound_of_fp32(tp, monkeypatch, dt, B, T, H, Dk, Dv):
+    import test_temporal_gpu
+    monkeypatch.setattr(test_temporal_gpu, 'decay_tol', fp32_tol)
+    for state in (False, True):
+        check_decay(tp, decay_case(B + T + Dk, dt, B, T, 1, H, Dk, Dv, ragged=B > 2, state=state, decays=[-0.001, 0.0, -0.1]))
