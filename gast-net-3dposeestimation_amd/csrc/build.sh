@@ -6,16 +6,15 @@ set -e
 HERE="$(cd "$(dirname "$0")" && pwd)"
 OUT="$HERE/../gast_hip/libgast_hip.so"
 HIPCC="${HIPCC:-/opt/rocm/bin/hipcc}"
-FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wno-comment"
+# No packed fp32 instructions (v_pk_add_f32 and its kin): hipcc makes them from scalar code by itself, and some of their forms have given wrong
+# results on this hardware.  (The host pass does not know the feature and says so.)
+FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wno-comment -Xclang -target-feature -Xclang -packed-fp32-ops"
 # ABLATION=1: profiling build of gemm_big.hip with the GAST_GEMM_BIG_ABLATE run-time switches compiled in (scripts/gemm_big_ablate.py)
 if [ -n "$ABLATION" ]; then FLAGS="$FLAGS -DGAST_GEMM_BIG_ABLATION"; fi
 # EXTRA_FLAGS="-DGAST_..." : experiment switches of single kernels (scripts/ab_variants.sh builds and times several variants on the GPU box)
 if [ -n "$EXTRA_FLAGS" ]; then FLAGS="$FLAGS $EXTRA_FLAGS"; fi
 HDRS="$HERE/common.h $HERE/gemm_big.h $HERE/bn_finalize.h $HERE/wgrad_common.h $HERE/seq_common.h $HERE/../../include/gast_hip.h"
 SRCS="gemm gemm_big gemm_bj wgrad wgrad_wide graph_ops norm_ops pack_ops optim_ops data_ops rotary layer_norm decay_attn"
-# The sequence operators are built without packed fp32 instructions (v_pk_*_f32), which hipcc makes from scalar code by itself.
-NO_PK="-Xclang -target-feature -Xclang -packed-fp32-ops"
-own_flags() { case "$1" in rotary|layer_norm|decay_attn) echo "$NO_PK" ;; esac; }
 # Two storage flavours of the SAME sources (common.h): libgast_hip.so keeps GAST_BF16 tensors as bfloat16, libgast_hip_f16.so
 # (-DGAST_H16_F16) as IEEE binary16 -- GAST_HIP_DTYPE=f16, the 16-bit mode that meets the north star's 1e-2 bound.  Same ABI.
 build_flavour() {   # $1 = object directory, $2 = output library, $3 = extra flags
@@ -23,12 +22,11 @@ build_flavour() {   # $1 = object directory, $2 = output library, $3 = extra fla
   mkdir -p "$BDIR"
   local pids=() names=()
   for f in $SRCS; do
-    local FF="$FL $(own_flags $f)"
-    want="$( (echo "$FF"; $HIPCC --version | head -2; cat "$HERE/$f.hip" $HDRS) | sha256sum | cut -d' ' -f1)"
+    want="$( (echo "$FL"; $HIPCC --version | head -2; cat "$HERE/$f.hip" $HDRS) | sha256sum | cut -d' ' -f1)"
     have="$(cat "$BDIR/$f.sha" 2>/dev/null || true)"
     if [ ! -f "$BDIR/$f.o" ] || [ "$want" != "$have" ]; then
       rm -f "$BDIR/$f.sha"
-      ( $HIPCC $FF -c "$HERE/$f.hip" -o "$BDIR/$f.o" && echo "$want" > "$BDIR/$f.sha" ) &
+      ( $HIPCC $FL -c "$HERE/$f.hip" -o "$BDIR/$f.o" && echo "$want" > "$BDIR/$f.sha" ) &
       pids+=($!)
       names+=($f)
     fi

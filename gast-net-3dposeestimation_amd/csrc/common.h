@@ -120,6 +120,15 @@ __device__ __forceinline__ float4 rnd4(float4 v, const bf16_t*) {
     return make_float4(bf2f(f2bf(v.x)), bf2f(f2bf(v.y)), bf2f(f2bf(v.z)), bf2f(f2bf(v.w)));
 }
 
+// fp32 values that are rounded to the storage type next: without this the binary16 build may fuse the arithmetic and the conversion into one
+// instruction that rounds once, in one kernel and not in another that has to give the same bits (the statement emits no instruction)
+__device__ __forceinline__ float4 in_fp32(float4 v) {
+#ifdef GAST_H16_F16
+    asm("" : "+v"(v.x), "+v"(v.y), "+v"(v.z), "+v"(v.w));
+#endif
+    return v;
+}
+
 // ---------------------------------------------------------------- dropout stream (see gast_dropout in gast_hip.h)
 __device__ __forceinline__ uint32_t hash32(uint32_t x) {
     x ^= x >> 16; x *= 0x7feb352du; x ^= x >> 15; x *= 0x846ca68bu; x ^= x >> 16;

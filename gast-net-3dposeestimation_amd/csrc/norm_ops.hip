@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(256) bn_bwd_apply_kernel(T* __restrict__ dz, i
             d.y = fmaf(a.y, d.y, fmaf(b.y, x.y, k.y));
             d.z = fmaf(a.z, d.z, fmaf(b.z, x.z, k.z));
             d.w = fmaf(a.w, d.w, fmaf(b.w, x.w, k.w));
-            st4(dz + r * lddz + c, d);
+            st4(dz + r * lddz + c, in_fp32(d));
         }
     }
 }
@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(256) bn_bwd_fused_kernel(const BnBwdFusedBatch
         d.y = fmaf(a.y, d.y, fmaf(kb.y, x.y, kc.y));
         d.z = fmaf(a.z, d.z, fmaf(kb.z, x.z, kc.z));
         d.w = fmaf(a.w, d.w, fmaf(kb.w, x.w, kc.w));
-        st4(dz + r * j.lddz + c, d);
+        st4(dz + r * j.lddz + c, in_fp32(d));
     }
 }
 
@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(256) bnrelu_bwd_mask_kernel(const T* dY, int l
                     d.z *= drop_mul(key, drop.thresh, drop.inv_keep, e0 + 2);
                     d.w *= drop_mul(key, drop.thresh, drop.inv_keep, e0 + 3);
                 }
-                d = rnd4(d, (const T*)nullptr);
+                d = rnd4(in_fp32(d), (const T*)nullptr);
                 st4(dz + r * lddz + c, d);
                 acc[0].x += d.x; acc[0].y += d.y; acc[0].z += d.z; acc[0].w += d.w;
                 acc[1].x = fmaf(d.x, x.x, acc[1].x); acc[1].y = fmaf(d.y, x.y, acc[1].y);
@@ -601,8 +601,8 @@ __global__ void __launch_bounds__(256) expand_bwd_kernel(const T* __restrict__ d
                     d0.z = fmaf(ca.z, d0.z, fmaf(cb.z, e0.z, ck.z)); d0.w = fmaf(ca.w, d0.w, fmaf(cb.w, e0.w, ck.w));
                     d1.x = fmaf(ca.x, d1.x, fmaf(cb.x, e1.x, ck.x)); d1.y = fmaf(ca.y, d1.y, fmaf(cb.y, e1.y, ck.y));
                     d1.z = fmaf(ca.z, d1.z, fmaf(cb.z, e1.z, ck.z)); d1.w = fmaf(ca.w, d1.w, fmaf(cb.w, e1.w, ck.w));
-                    d0 = rnd4(d0, (const T*)nullptr);
-                    d1 = rnd4(d1, (const T*)nullptr);
+                    d0 = rnd4(in_fp32(d0), (const T*)nullptr);
+                    d1 = rnd4(in_fp32(d1), (const T*)nullptr);
                 }
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {

@@ -18,7 +18,7 @@ hipcc = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
 print('%-78s %5s %5s %6s %6s %8s %8s' % ('kernel', 'vgpr', 'w/SIMD', 'vspill', 'sspill', 'scratch', 'lds'))
 for f in files:
     with tempfile.NamedTemporaryFile(suffix='.s') as tmp:
-        r = subprocess.run([hipcc, '--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-Wno-comment', '-S', '--cuda-device-only', '-o', tmp.name, f],
+        r = subprocess.run([hipcc, '--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-Wno-comment', '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops', '-S', '--cuda-device-only', '-o', tmp.name, f],
                            capture_output=True, text=True, cwd=CSRC)
         if r.returncode:
             print('%s: %s' % (f, r.stderr.splitlines()[-1] if r.stderr else 'failed'))
