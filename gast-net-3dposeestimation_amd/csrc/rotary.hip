@@ -55,9 +55,10 @@ __global__ void __launch_bounds__(NTHR) rotary_kernel(const RotaryArgs a) {
         const double pos = a.pos64 ? (double)((const int64_t*)a.pos)[at] : (double)((const int32_t*)a.pos)[at];
         double turns = pos * a.freqs[f] * 0.15915494309189533577;       // 1 / (2 pi)
         turns -= rint(turns);
+        const float near = (float)turns, rest = 6.28318531f * (float)(turns - (double)near);       // (what fp32 leaves of the angle: small sines keep their bits)
         float s, c;
-        sincospif(2.f * (float)turns, &s, &c);
-        cs[i] = make_float2(c * a.scale, s * a.scale * a.sign);
+        sincospif(2.f * near, &s, &c);
+        cs[i] = make_float2(fmaf(-rest, s, c) * a.scale, fmaf(rest, c, s) * a.scale * a.sign);
     }
     __syncthreads();
     // units of a row: the rotated ones, then the copied tail in pieces of the same size
@@ -170,7 +171,7 @@ extern "C" int gast_rotary_multi(int dtype, const gast_rotary_job* jobs, int n, 
     const int maxsplit = (int)(((long)J * maxH + a.RL - 1) / a.RL);
     long by = 1024 / (bx * n);
     by = by < 1 ? 1 : by > maxsplit ? maxsplit : by;
-// few heads and many tokens: a block turns all jobs by the cosines it has made (497k tokens of 2 + 2 heads of 14 channels, fp32: 237 -> 140 us
+    // few heads and many tokens: a block turns all jobs by the cosines it has made (497k tokens of 2 + 2 heads of 14 channels, fp32: 237 -> 140 us
     // both ways, with more tokens a block).  With many heads the cosines are cheap and blocks of one job are faster (32 + 8 heads of 128: 75 against 67 us).
     const bool share = 4L * R2 > (long)J * maxH * U && bx * by >= 1024;
     const dim3 grid((unsigned)bx, (unsigned)by, (unsigned)(share ? 1 : n));

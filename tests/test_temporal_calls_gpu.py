@@ -1,4 +1,6 @@
 """Calls that the documentation of gast_hip.temporal allows, beside those of sizes and types."""
+import math
+
 import pytest
 import torch
 from test_temporal_gpu import check_decay, decay_case
@@ -63,3 +65,21 @@ def test_sequences_of_one_chunk_that_go_on_from_a_state(tp, dt, T, Dk, Dv):
     for _ in range(3):
         again = check_decay(tp, c)
         assert all(torch.equal(first[n], again[n]) for n in first)
+
+
+@pytest.mark.parametrize('layout', ['half', 'pairs'])
+@pytest.mark.parametrize('around', [0.0, 0.25, 0.5, 0.75, 1.0, 1000.5])
+def test_rotations_near_quarter_turns_keep_the_bits_of_what_is_small(tp, layout, around):
+    """(1, 0) turned by `around` -+ 2^-20 turns: cosine and sine are each good to 2 steps of fp32 (4 u) of themselves, a correction, the scale
+    and the product with 1 round once more (3 u), and the angle is off by 2 pi turns 2^-51; 8 u of the value, where u is 2^-24"""
+    g = torch.Generator().manual_seed(int(around * 4))
+    turns = around + (torch.rand(64, generator=g, dtype=torch.float64) - 0.5) * 2.0 ** -19
+    f = turns * (2 * math.pi)
+    x = torch.zeros(1, 2, 1, 1, 128)
+    a = torch.arange(0, 128, 2) if layout == 'pairs' else torch.arange(64)
+    b = a + 1 if layout == 'pairs' else a + 64
+    x[..., a] = 1.0
+    y = tp.rotary(x.cuda(), torch.tensor([1, -1]).cuda(), f.cuda(), interleaved=layout == 'pairs')[0, :, 0, 0].double().cpu()
+    for t, sign in ((0, 1), (1, -1)):
+        for at, ref in ((a, torch.cos(sign * f)), (b, torch.sin(sign * f))):
+            assert torch.all((y[t, at] - ref).abs() <= 8 * 2.0 ** -24 * ref.abs() + 6.3 * (around + 1) * 2.0 ** -51)
