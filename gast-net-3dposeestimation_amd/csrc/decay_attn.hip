@@ -32,11 +32,12 @@ namespace {
 // against 183 us, with gradients 585 against 705), 5 - 12 % with 64, but what is left of terms that nearly cancel is then off by 2^-17 of the terms.
 //
 // What bounds it, on a full card (two waves a SIMD, 1024 tokens, without gradients; a copy of the same bytes takes 112 us at 16 bits, 224 fp32):
-//   bf16  1024 heads of 64: 128 us, memory (4.2 TB/s); 512 of 128: 145 us, issue (586 vector, 52 matrix and 54 LDS instructions a wave and chunk:
+//   bf16  1024 heads of 64: 136 us, memory (3.9 TB/s); 512 of 128: 183 us, issue (823 vector, 62 matrix and 54 LDS instructions a wave and chunk:
 //         the splits into parts are most of them)
-//   fp16  64: 170 us, 128: 205 us: issue, both sides of a product are split
-//   fp32  2048 heads of 32: 327 us and 1024 of 64: 300 us, memory and LDS; 512 of 128: 490 - 540 us, of which 355 are matrix instructions
-// 16 heads of 128 channels and 32768 tokens (bf16) are cut into 32 segments: 80 us of sums, 14 of joining them, 175 of outputs.
+//   fp16  64: 181 us, 128: 257 us: issue, both sides of a product are split
+//   fp32  2048 heads of 32: 314 us and 1024 of 64: 309 us, memory and LDS; 512 of 128: 480 us, of which 355 are matrix instructions (208 of 64
+//         cycles a wave and chunk)
+// 16 heads of 128 channels and 32768 tokens (bf16) are cut into 32 segments: 80 us of sums, 14 of joining them, 177 of outputs.
 constexpr int CT = 32;               // tokens of a chunk
 constexpr int TS = CT + 4;           // row pitch of the turned tiles (elements): rows start 18 / 36 banks apart, no two of a read collide
 
@@ -815,7 +816,7 @@ int check(const gast_decay_args* p) {
 // block: a cut reads two of the tensors twice (half a chunk's work for each chunk), hands a state of D x D fp32 over four times for each segment
 // (as many bytes as D / 16 chunks of 16-bit tokens have, D / 32 of fp32), and has two launches more (about 6 chunks' time, 4 of the longer fp32
 // ones).  A CU runs eight waves' worth of blocks at once, two to a SIMD; a last round that is not full still takes half of one.
-// Measured, uncut and cut: 16 heads of 128 channels and 32768 tokens (bf16, forward) 1937 us in two segments, 272 in 32; forward and backward in fp32,
+// Measured, uncut and cut: 16 heads of 128 channels and 32768 tokens (bf16, forward) 2234 us in two segments, 313 in 32; forward and backward in fp32,
 // 12 heads of 16 and 530 tokens 203 and 44 in 17, 128 heads of 64 and 362 tokens 189 and 140 in 6.
 struct Cut { int dp, nseg, L; };
 Cut cut(int dtype, long heads, int T, int Dk, int Dv) {

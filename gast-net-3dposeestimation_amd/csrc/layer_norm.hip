@@ -392,6 +392,8 @@ __global__ void __launch_bounds__(1024) norm_wsum_kernel(const float* __restrict
 
 // How a row is held: vectors of ve values, G lanes, NC vectors a lane (at most MAXV values); G = 0: the long kernels.
 // The narrowest group that can hold the row: 32 lanes, a wave, then 256 .. 1024 threads.
+// A row has 32 lanes at least, and a width that is no multiple of a vector has narrower ones, which is slow for short rows and for odd widths of
+// 16 bits (64 MB a tensor, forward, fp32 / bf16: C = 8 0.9 / 0.4 TB/s, 32 3.3 / 1.4, 64 5.3 / 2.7, 87 4.0 / 2.2, 128 6.4 / 4.8, 4095 5.8 / 1.8, 4096 6.3 / 5.9).
 struct Shape { int ve, G, NC; };
 
 Shape shape_of(int C, int ve) {
@@ -420,8 +422,8 @@ int row_align(const void* p, long ld, int es, int ve) {
 }
 
 constexpr int LONG_BLOCKS = 256;
-// blocks of the backward pass: each leaves a partial row of 2 C sums, so there are no more than one for every 64 KB or so it reads --
-// the partial rows stay below an eighth of the tensors -- and no more than fill the card
+// blocks of the backward pass: each leaves a partial row of 2 C sums (8 C bytes), so there are no more than one for every 64 C bytes or so of
+// S, dY and dX -- the partial rows stay below an eighth of the tensors -- and no more than fill the card
 long bwd_blocks(long rows, int C, int es, int G) {
     if (!G) return rows < LONG_BLOCKS ? rows : LONG_BLOCKS;
     const int gpb = G > 256 ? 1 : 256 / G;

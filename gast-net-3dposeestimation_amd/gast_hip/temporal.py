@@ -78,8 +78,8 @@ def decay_attention(q, k, v, log_decay, state=None, lengths=None, scale=None, re
     exp(log_decay * min(tokens, 32)) has to be a finite fp32 number), not trained: one that requires grad is refused where autograd records.
     state: S before the first token, (B, J, H, Dk, Dv) float32 (J = 1 for plain sequences; None: zero).  lengths: (B,) tokens of each clip,
     clamped to 0 .. T (None: T); outputs and gradients behind a clip's end are zero, whatever stands there in the inputs.  scale: Dk ** -0.5.
-    Returns o, or (o, state behind the last token of each clip) with return_state=True.  Differentiable in q, k, v and state; S is held in
-    fp32 throughout."""
+    Returns o, or (o, state behind the last token of each clip) with return_state=True.  Differentiable in q, k, v and state.  Whatever the
+    type, scores, sums and S are fp32 and enter products with all their bits; o and the gradients are rounded to the type at the end."""
     out = _temporal.decay_attention(q, k, v, log_decay, state, lengths, scale, return_state)
     return tuple(out) if return_state else out[0]
 
@@ -99,8 +99,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
 
 
 def add_layer_norm(x, residual, weight=None, bias=None, eps=1e-5, drop=None, salt=0):
-    """s = residual + dropout(x), y = layer_norm(s), in one pass: returns (y, s).  s is rounded to the tensors' type and y is the norm of
-    the rounded values, so both match what the next layer reads.  drop: gast_hip.binding.Dropout(seed, *dropout_params(p)) -- the library's
+    """s = residual + dropout(x), y = layer_norm(s), in one pass: returns (y, s).  s is made in fp32 and rounded to the tensors' type,
+    and y is the norm of the rounded values, so both match what the next layer reads.  drop: gast_hip.binding.Dropout(seed, *dropout_params(p)) -- the library's
     counter stream at tensor `salt`, element by element in the order of x's axes; its mask is not stored but made again in the backward
     pass from the seed tensor, which must not change in between -- or None.  Differentiable in x, residual, weight and bias."""
     if drop is None:

@@ -509,7 +509,7 @@ typedef struct { gast_seq x, y; int H; } gast_rotary_job;
 int gast_rotary_multi(int dtype, const gast_rotary_job* jobs, int n, int B, int T, int J, int D, int R, int interleaved, const void* positions,
                       int pos64, long pos_b, long pos_t, const double* freqs, float scale, int backward, gast_stream_t stream);
 
-/* Layer norm of the rows of S, or of S = residual + drop(X) (residual != null; S is then written, rounded to the activation type, and
+/* Layer norm of the rows of S, or of S = residual + drop(X) (residual != null; S is then made in fp32 and written, rounded to the activation type, and
  * the norm is of the rounded values): y = (s - mean) * rstd * gamma + beta, rstd = 1 / sqrt(var + eps).  gamma, beta: fp32 or null.
  * mean, rstd: fp32 [rows], or null where no backward pass follows.  Dropout: the library's stream of tensor `salt` at element r * C + c
  * (beyond 2^33 elements the high word enters the key); use_drop needs a residual.  ld*: row strides in elements. */
@@ -527,7 +527,8 @@ long gast_layer_norm_bwd_ws_floats(long rows, int C);
 /* Causal linear attention with a decay for each head, lambda_h = exp(log_decay[h]):
  *   S_t = lambda S_(t-1) + k_t v_t',   o_t = scale q_t' S_t,   t < lengths[b] (null: T; clamped to 0 .. T)
  * S_(-1) = state ([B][J][H][Dk][Dv] fp32; null: zero), state_out (null: not wanted) = S behind the last token.  Outputs behind a
- * sequence's end are zero.  Outputs overlap no input.  An infinity or NaN of a token reaches what sees the token and nothing else.
+ * sequence's end are zero.  exp(n log_decay[h]) has to be finite for n up to the sequence's tokens or 32.  Scores, sums and S are fp32
+ * for every dtype.  Outputs overlap no input.  An infinity or NaN of a token reaches what sees the token and nothing else.
  * Dk, Dv <= GAST_DECAY_MAX_D. */
 #define GAST_DECAY_MAX_D 128
 typedef struct {

@@ -45,3 +45,28 @@ def test_no_packed_fp32_instructions(h16, tmp_path):
         assert not found, '%d in source %d' % (len(found), i)
         objects += 1
     assert objects >= 13
+
+
+def test_the_load_hazard_screens_hold_for_the_flags_of_the_build(tmp_path):
+    """scripts/asm_load_hazard.py on the sources with loads in inline asm, compiled as csrc/build.sh compiles them (gemm_big and wgrad_wide, which
+    take minutes, with GAST_TEST_ASM_SCAN_ALL=1)"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    csrc = os.path.join(root, 'gast-net-3dposeestimation_amd', 'csrc')
+    hipcc = '/opt/rocm/bin/hipcc'
+    if not os.path.exists(hipcc):
+        pytest.skip('no hipcc')
+    with open(os.path.join(csrc, 'build.sh')) as f:
+        flags = re.search(r'^FLAGS="([^"$]*)"', f.read(), re.M).group(1).split()
+    assert '-packed-fp32-ops' in flags
+    names = ['gemm', 'wgrad', 'gemm_bj'] + (['gemm_big', 'wgrad_wide'] if os.environ.get('GAST_TEST_ASM_SCAN_ALL') else [])
+    runs = []
+    for n in names:
+        out = str(tmp_path / (n + '.s'))
+        runs.append((n, out, subprocess.Popen([hipcc] + flags + ['-S', '--cuda-device-only', os.path.join(csrc, n + '.hip'), '-o', out], stdout=subprocess.DEVNULL,
+                                              stderr=subprocess.PIPE)))
+    for n, out, p in runs:
+        _, err = p.communicate(timeout=900)
+        assert p.returncode == 0, '%s.hip did not compile: %s' % (n, err.decode()[-800:])
+        for mode, none in (('--strict', '0 suspicious instruction(s)'), ('--sgpr', '0 VALU->SGPR->VMEM hazard(s)')):
+            r = subprocess.run(['python3', os.path.join(root, 'scripts', 'asm_load_hazard.py'), mode, out], capture_output=True, text=True)
+            assert r.returncode == 0 and none in r.stdout, '%s.hip: %s' % (n, r.stdout[-1500:])
